@@ -9,6 +9,7 @@ Three operators of one train-and-forecast run:
 `run` computes a case in elementary torch operations (`own` false) or through regcn_amd's entry
 points (`own` true); `exact` computes it once more in 64 bits from the operator's definition.
 """
+import importlib
 import math
 import os
 import sys
@@ -174,8 +175,9 @@ def prepare(case, seed):
         path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "re-gcn_amd")
         if path not in sys.path:
             sys.path.insert(0, path)
-        from regcn_amd import autograd, muon, ranking
-        state["calls"] = {"lookup": autograd.embedding, "orth": muon.orthogonalize, "sample": ranking.sample}
+        module, name = {"lookup": ("autograd", "embedding"), "orth": ("muon", "orthogonalize"),
+                        "sample": ("ranking", "sample")}[case["op"]]
+        state["call"] = getattr(importlib.import_module("regcn_amd." + module), name)
         if case["op"] == "lookup" and case["grad"]:
             state["table"].requires_grad_(True)
     return state
@@ -187,7 +189,7 @@ def run(state):
 
 
 def _run_own(st):
-    case, call = st["case"], st["calls"][st["case"]["op"]]
+    case, call = st["case"], st["call"]
     if case["op"] == "lookup":
         if not case["grad"]:
             with torch.no_grad():
