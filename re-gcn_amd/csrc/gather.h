@@ -101,8 +101,8 @@ struct WFrag {
   __device__ __forceinline__ f4 apply(f4 xs) const {
     if constexpr (S == 1) return xs * w[0];
     else if constexpr (S == 2) {
-      // (m0, m1) = x0 (W00, W01) + x1 (W10, W11): packed-fp32 pairs straight from the
-      // loaded quads (v_pk_mul / v_pk_fma with a broadcast operand, no repacking moves)
+      // (m0, m1) = x0 (W00, W01) + x1 (W10, W11): pairs straight from the
+      // loaded quads (no repacking moves)
       const f2 lo = w[0].zw * xs.y + w[0].xy * xs.x;
       const f2 hi = w[1].zw * xs.w + w[1].xy * xs.z;
       return f4{lo.x, lo.y, hi.x, hi.y};
