@@ -33,6 +33,11 @@ extern "C" {
 #define REGCN_EINVAL (-1)
 #define REGCN_ENOTSUP (-2)
 
+/* Element types of the entry points that take them (`dtype`). */
+#define REGCN_F32 0
+#define REGCN_BF16 1
+#define REGCN_F16 2
+
 /* Snapshot work lists built by the host (re-gcn_amd/regcn_amd/graph.py):
  * chunks: int32[n_chunks][4] = {row, edge_begin, edge_end, slot}; slot < 0 means
  *         the row is finished by that chunk, slot >= 0 names its partial row.
@@ -835,6 +840,19 @@ int regcn_hyp_ce_bwd_f32(const float* q, const float* cand, const float* bias, c
                          const float* margin, const int32_t* target, const float* lse, const float* grad_loss,
                          int32_t B, int32_t N, int32_t d, float c, int32_t flags, float* coef, float* rsum,
                          float* csum, void* stream);
+
+/* ---- Embedding rows ------------------------------------------------------------------- */
+/* out[i, :] = scale * table[idx[i], :], one rounding to `dtype`.  table: V rows of d elements,
+ * `ld` elements apart (any element-aligned address); idx: n int32 (idx_wide = 0) or int64 indices;
+ * out: n x d contiguous.  An index outside [0, V) reads nothing and leaves a NaN row. */
+int regcn_embedding(const void* table, int64_t ld, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d,
+                    int32_t dtype, float scale, void* out, void* stream);
+/* Its gradient: out[v, :] = scale * sum of grad[i, :] over the tokens i with idx[i] = v, for every
+ * v in [0, V) (zeros where there is none).  fp32 sums in a fixed order (the same bits on every
+ * call), one rounding to `dtype`.  Tokens equal to `pad` (>= 0) or outside [0, V) are left out. */
+int64_t regcn_embedding_grad_workspace_bytes(int64_t n, int64_t V, int32_t d);
+int regcn_embedding_grad(const void* grad, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d, int64_t pad,
+                         int32_t dtype, float scale, void* out, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -783,4 +783,14 @@ int regcn_snapshot_row_type_order_i32(int32_t V, int32_t E, int32_t R2, const in
   return row_type_order(V, E, R2, rowptr, col_src, col_type, out_src, out_type, workspace, ws_bytes, ST(s));
 }
 
+int regcn_embedding(const void* table, int64_t ld, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d,
+                    int32_t dtype, float scale, void* out, void* s) {
+  return embedding(table, ld, idx, idx_wide, n, V, d, dtype, scale, out, ST(s));
+}
+int64_t regcn_embedding_grad_workspace_bytes(int64_t n, int64_t V, int32_t d) { return embedding_grad_ws_bytes(n, V, d); }
+int regcn_embedding_grad(const void* grad, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d, int64_t pad,
+                         int32_t dtype, float scale, void* out, void* workspace, size_t ws_bytes, void* s) {
+  return embedding_grad(grad, idx, idx_wide, n, V, d, pad, dtype, scale, out, workspace, ws_bytes, ST(s));
+}
+
 }  // extern "C"

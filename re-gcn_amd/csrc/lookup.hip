@@ -1,0 +1,459 @@
+// Embedding lookup with scaling and its gradient by sorted tokens.
+//
+//   out[i, :]   = s * table[idx[i], :]
+//   dtable[v, :] = s * sum over the tokens i with idx[i] = v, in ascending i, of g[i, :]
+//
+// An index outside [0, V) reads nothing: its output row is NaN and it joins no gradient row.
+// Tokens of `pad` join no gradient row either.
+//
+// Both directions are bound by memory: the forward reads and writes n rows, the gradient reads
+// n rows of g and writes all V rows of dtable once (zeros included; no clearing pass).
+//
+// The gradient first sorts the tokens by index (stable), so that each row's tokens are one run of
+// sorted positions, then sums the runs in a fixed order: no atomics, the same bits on every call.
+//   * up to RANK_MAX tokens one launch ranks each token by counting the keys before it;
+//   * more take least-significant-digit radix passes of 10 bits (two launches a pass).
+// A run of any length is summed in three levels: whole 64-token blocks inside a run are summed by
+// k_block_sums, whole groups of 64 such blocks by k_group_sums, and the row's thread adds its ends
+// to those.  Sums are fp32; a 16-bit type is rounded once, at the store.
+#include "elem.h"
+#include "regcn_internal.h"
+
+namespace regcn {
+namespace {
+
+constexpr int RANK_MAX = 16384;    // tokens ranked by counting (their keys in 64 KB of LDS)
+constexpr int BLK = 64;            // sorted positions of a block
+constexpr int GRP = BLK * BLK;     // ... of a group of blocks
+constexpr int RADIX_BITS = 10, BINS = 1 << RADIX_BITS;
+constexpr int MAX_TILES = 256;     // radix tiles (a workgroup each)
+constexpr int SORT_THR = 1024, SORT_WAVES = SORT_THR / WAVE;
+constexpr int ROW_THR = 256;
+
+struct Tokens {
+  const void* idx;
+  int wide;      // idx is int64
+  int64_t n, V, pad;
+};
+
+// The sort key: the row, or V for a token without one.
+__device__ __forceinline__ uint32_t token_key(const Tokens& t, int64_t i) {
+  const int64_t v = t.wide ? ((const int64_t*)t.idx)[i] : (int64_t)((const int32_t*)t.idx)[i];
+  return (uint32_t)(v < 0 || v >= t.V || v == t.pad ? t.V : v);
+}
+
+// ------------------------------------------------------------------------------------ forward
+template <typename T>
+__global__ __launch_bounds__(ROW_THR) void k_lookup(const T* __restrict__ table, int64_t ld, Tokens t, int d,
+                                                    float scale, T* __restrict__ out) {
+  constexpr int VE = Piece<T>::VE;
+  const int C = (d + VE - 1) / VE;
+  const int64_t total = t.n * C;
+  for (int64_t it = (int64_t)blockIdx.x * ROW_THR + threadIdx.x; it < total; it += (int64_t)gridDim.x * ROW_THR) {
+    const int64_t i = total <= 0x7fffffff ? (int64_t)((uint32_t)it / (uint32_t)C) : it / C;
+    const int c0 = (int)(it - i * C) * VE;
+    const int m = d - c0;
+    const int64_t v = t.wide ? ((const int64_t*)t.idx)[i] : (int64_t)((const int32_t*)t.idx)[i];
+    float x[VE];
+    if (v >= 0 && v < t.V) {
+      load_piece<T>(x, table + v * ld + c0, m);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] *= scale;
+    store_piece<T>(out + i * d + c0, x, m);
+  }
+}
+
+// --------------------------------------------------------------------------------------- sort
+// Runs of every row cleared: {first, end} = {0, 0}.
+__device__ __forceinline__ void clear_runs(int2* runs, int64_t V) {
+  for (int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; v < V; v += (int64_t)gridDim.x * blockDim.x)
+    runs[v] = make_int2(0, 0);
+}
+
+// One launch for n <= RANK_MAX: a workgroup ranks 64 tokens, each of its 16 waves counting a
+// sixteenth of the keys: rank = #{key_j < key} + #{j < i, key_j = key}.  n^2 compares spread over
+// the card: 16 million (n = 4096) take about 2 us, against 3 dependent sort passes on one CU.
+__global__ __launch_bounds__(SORT_THR) void k_rank(Tokens t, int32_t* __restrict__ perm, uint32_t* __restrict__ skey,
+                                                   int2* __restrict__ runs) {
+  __shared__ __align__(16) uint32_t keys[RANK_MAX];
+  __shared__ int part[SORT_WAVES][WAVE];
+  clear_runs(runs, t.V);
+  const int n = (int)t.n, i0 = blockIdx.x * WAVE;
+  if (i0 >= n) return;
+  const int npad = (n + 255) & ~255;  // whole uint4 per wave stripe; the padding never counts
+  for (int j = threadIdx.x; j < npad; j += SORT_THR) keys[j] = j < n ? token_key(t, j) : 0xffffffffu;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int i = i0 + lane;
+  const uint32_t k = keys[min(i, n - 1)];
+  const int per = npad / SORT_WAVES;  // a multiple of 16
+  const int j0 = w * per, j1 = j0 + per;
+  int cnt = 0;
+  // keys of the lower positions count when <= k, those of the higher ones when < k; the 64
+  // positions around i0 are told apart one by one
+  const int lo = min(j1, i0), hi = max(j0, i0 + WAVE);
+  for (int j = j0; j < lo; j += 4) {
+    const uint4 q = *(const uint4*)(keys + j);
+    cnt += (q.x <= k) + (q.y <= k) + (q.z <= k) + (q.w <= k);
+  }
+  for (int j = max(j0, i0); j < min(j1, i0 + WAVE); ++j) cnt += keys[j] < k || (keys[j] == k && j < i);
+  for (int j = hi; j < j1; j += 4) {
+    const uint4 q = *(const uint4*)(keys + j);
+    cnt += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
+  }
+  part[w][lane] = cnt;
+  __syncthreads();
+  if (w == 0 && i < n) {
+    int r = 0;
+#pragma unroll
+    for (int u = 0; u < SORT_WAVES; ++u) r += part[u][lane];
+    perm[r] = i;
+    skey[r] = k;
+  }
+}
+
+// Radix pass, first half: hist[tile][bin] of the pass's digit.
+__global__ __launch_bounds__(SORT_THR) void k_hist(Tokens t, const uint32_t* __restrict__ key_in, int shift, int64_t tile,
+                                                   uint32_t* __restrict__ hist, int2* __restrict__ runs) {
+  __shared__ uint32_t h[BINS];
+  if (runs) clear_runs(runs, t.V);
+  for (int b = threadIdx.x; b < BINS; b += SORT_THR) h[b] = 0;
+  __syncthreads();
+  const int64_t p0 = (int64_t)blockIdx.x * tile, p1 = min(p0 + tile, t.n);
+  for (int64_t p = p0 + threadIdx.x; p < p1; p += SORT_THR) {
+    const uint32_t k = key_in ? key_in[p] : token_key(t, p);
+    atomicAdd(&h[(k >> shift) & (BINS - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < BINS; b += SORT_THR) hist[(int64_t)blockIdx.x * BINS + b] = h[b];
+}
+
+// Second half: each workgroup finds where its tile's bins begin from the whole histogram, then
+// places its tokens in order (stable): a wave ranks 64 consecutive tokens at a time by matching
+// digits across its lanes, the waves of a 1024-token step in wave order.
+__global__ __launch_bounds__(SORT_THR) void k_scatter(Tokens t, const uint32_t* __restrict__ key_in,
+                                                      const int32_t* __restrict__ val_in, int shift, int64_t tile,
+                                                      const uint32_t* __restrict__ hist, uint32_t* __restrict__ key_out,
+                                                      int32_t* __restrict__ val_out) {
+  __shared__ uint32_t base[BINS];                  // where the next token of a bin goes
+  __shared__ uint16_t wcnt[SORT_WAVES][BINS];      // a step's tokens per wave and bin
+  __shared__ uint32_t wsum[SORT_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tiles = gridDim.x, me = blockIdx.x;
+  static_assert(BINS == SORT_THR, "a thread per bin");
+  uint32_t before = 0, total = 0;
+  for (int s = 0; s < tiles; ++s) {
+    const uint32_t c = hist[(int64_t)s * BINS + tid];
+    before += s < me ? c : 0;
+    total += c;
+  }
+  // exclusive scan of the totals over the bins
+  uint32_t x = total;
+#pragma unroll
+  for (int o = 1; o < WAVE; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) wsum[w] = x;
+  __syncthreads();
+  uint32_t wbase = 0;
+  for (int u = 0; u < w; ++u) wbase += wsum[u];
+  base[tid] = wbase + x - total + before;
+  const int64_t p0 = (int64_t)me * tile, p1 = min(p0 + tile, t.n);
+  for (int64_t s = p0; s < p1; s += SORT_THR) {
+    for (int u = 0; u < SORT_WAVES; ++u) wcnt[u][tid] = 0;
+    __syncthreads();
+    const int64_t p = s + tid;
+    const bool ok = p < p1;
+    uint32_t k = 0, dig = 0;
+    int32_t val = 0;
+    if (ok) {
+      k = key_in ? key_in[p] : token_key(t, p);
+      val = val_in ? val_in[p] : (int32_t)p;
+      dig = (k >> shift) & (BINS - 1);
+    }
+    uint64_t same = __ballot(ok);
+#pragma unroll
+    for (int b = 0; b < RADIX_BITS; ++b) {
+      const uint64_t m = __ballot((dig >> b) & 1);
+      same &= (dig >> b) & 1 ? m : ~m;
+    }
+    const uint32_t in_wave = __popcll(same & ((1ull << lane) - 1));
+    if (ok && in_wave == 0) wcnt[w][dig] = (uint16_t)__popcll(same);
+    __syncthreads();
+    if (ok) {
+      uint32_t r = base[dig] + in_wave;
+      for (int u = 0; u < w; ++u) r += wcnt[u][dig];
+      key_out[r] = k;
+      val_out[r] = val;
+    }
+    __syncthreads();
+    uint32_t add = 0;
+    for (int u = 0; u < SORT_WAVES; ++u) add += wcnt[u][tid];
+    base[tid] += add;
+    __syncthreads();
+  }
+}
+
+// --------------------------------------------------------------------------------------- sums
+// acc += rows src[0..cnt) of width-d pieces; src[j] = base + row(j) * d.
+template <typename T, typename Row>
+__device__ __forceinline__ void add_rows(float (&acc)[Piece<T>::VE], const T* __restrict__ base, int64_t d, int c0, int m,
+                                         int cnt, Row row) {
+  constexpr int VE = Piece<T>::VE, U = 4;
+  int j = 0;
+  for (; j + U <= cnt; j += U) {
+    float x[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_piece<T>(x[u], base + row(j + u) * d + c0, m);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] += x[u][e];
+  }
+  for (; j < cnt; ++j) {
+    float x[VE];
+    load_piece<T>(x, base + row(j) * d + c0, m);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] += x[e];
+  }
+}
+
+// A partial row piece (VE floats of the fp32 partial sums).
+template <int VE>
+__device__ __forceinline__ void add_partials(float (&acc)[VE], const float* __restrict__ part, int64_t dp, int c0, int cnt) {
+  for (int j = 0; j < cnt; ++j) {
+    const f4* q = reinterpret_cast<const f4*>(part + j * dp + c0);
+#pragma unroll
+    for (int h = 0; h < VE / 4; ++h) {
+      const f4 v = q[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * h + e] += v[e];
+    }
+  }
+}
+
+template <int VE>
+__device__ __forceinline__ void store_partial(float* __restrict__ part, const float (&acc)[VE]) {
+  f4* q = reinterpret_cast<f4*>(part);
+#pragma unroll
+  for (int h = 0; h < VE / 4; ++h) q[h] = f4{acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
+}
+
+// Per 64 sorted positions: the ends of the runs that lie in them, and their sum where all 64
+// belong to one row.  dp: the partial rows' width (d rounded up to whole pieces).
+template <typename T>
+__global__ __launch_bounds__(ROW_THR) void k_block_sums(const T* __restrict__ g, const int32_t* __restrict__ perm,
+                                                        const uint32_t* __restrict__ skey, int64_t n, int64_t V, int d,
+                                                        int64_t dp, int2* __restrict__ runs, float* __restrict__ part) {
+  constexpr int VE = Piece<T>::VE;
+  const int64_t p0 = (int64_t)blockIdx.x * BLK;
+  if (threadIdx.x < BLK) {
+    const int64_t p = p0 + threadIdx.x;
+    if (p < n) {
+      const uint32_t k = skey[p];
+      if (k < V) {
+        if (p == 0 || skey[p - 1] != k) runs[k].x = (int)p;
+        if (p == n - 1 || skey[p + 1] != k) runs[k].y = (int)p + 1;
+      }
+    }
+  }
+  if (p0 + BLK > n) return;
+  const uint32_t k0 = skey[p0];
+  if (k0 >= V || skey[p0 + BLK - 1] != k0) return;
+  const int C = (int)(dp / VE);
+  for (int c = threadIdx.x; c < C; c += ROW_THR) {
+    float acc[VE] = {};
+    add_rows<T>(acc, g, d, c * VE, d - c * VE, BLK, [&](int j) { return (int64_t)perm[p0 + j]; });
+    store_partial<VE>(part + (int64_t)blockIdx.x * dp + c * VE, acc);
+  }
+}
+
+// Per 4096 sorted positions of one row: the sum of its 64 block sums.
+template <int VE>
+__global__ __launch_bounds__(ROW_THR) void k_group_sums(const uint32_t* __restrict__ skey, int64_t V, int64_t dp,
+                                                        const float* __restrict__ part, float* __restrict__ part2) {
+  const int64_t p0 = (int64_t)blockIdx.x * GRP;
+  const uint32_t k0 = skey[p0];
+  if (k0 >= V || skey[p0 + GRP - 1] != k0) return;
+  const int C = (int)(dp / VE);
+  for (int c = threadIdx.x; c < C; c += ROW_THR) {
+    float acc[VE] = {};
+    add_partials<VE>(acc, part + (int64_t)blockIdx.x * BLK * dp, dp, c * VE, BLK);
+    store_partial<VE>(part2 + (int64_t)blockIdx.x * dp + c * VE, acc);
+  }
+}
+
+// Every row of dtable, once: s * (tokens before the first whole block + block sums + group sums +
+// block sums + tokens after the last whole block), zero for a row without tokens.
+template <typename T>
+__global__ __launch_bounds__(ROW_THR) void k_row_grads(const T* __restrict__ g, const int32_t* __restrict__ perm,
+                                                       const int2* __restrict__ runs, const float* __restrict__ part,
+                                                       const float* __restrict__ part2, int64_t V, int d, int64_t dp,
+                                                       int rows_per_wg, float scale, T* __restrict__ out) {
+  constexpr int VE = Piece<T>::VE;
+  const int C = (int)(dp / VE);
+  const int64_t v0 = (int64_t)blockIdx.x * rows_per_wg;
+  const int rows = (int)min((int64_t)rows_per_wg, V - v0);
+  for (int it = threadIdx.x; it < rows * C; it += ROW_THR) {
+    const int r = (int)((uint32_t)it / (uint32_t)C);
+    const int c0 = (it - r * C) * VE, m = d - c0;
+    const int2 run = runs[v0 + r];
+    float acc[VE] = {};
+    if (run.x < run.y) {
+      const int b0 = (run.x + BLK - 1) / BLK, b1 = run.y / BLK;  // whole blocks [b0, b1)
+      const auto token = [&](int p) {
+        return [=](int j) { return (int64_t)perm[p + j]; };
+      };
+      if (b0 >= b1) {
+        add_rows<T>(acc, g, d, c0, m, run.y - run.x, token(run.x));
+      } else {
+        add_rows<T>(acc, g, d, c0, m, b0 * BLK - run.x, token(run.x));
+        const int g0 = (b0 + BLK - 1) / BLK, g1 = b1 / BLK;  // whole groups [g0, g1)
+        if (g0 >= g1) {
+          add_partials<VE>(acc, part + b0 * dp, dp, c0, b1 - b0);
+        } else {
+          add_partials<VE>(acc, part + b0 * dp, dp, c0, g0 * BLK - b0);
+          add_partials<VE>(acc, part2 + g0 * dp, dp, c0, g1 - g0);
+          add_partials<VE>(acc, part + (int64_t)g1 * BLK * dp, dp, c0, b1 - g1 * BLK);
+        }
+        add_rows<T>(acc, g, d, c0, m, run.y - b1 * BLK, token(b1 * BLK));
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] *= scale;
+    }
+    store_piece<T>(out + (v0 + r) * d + c0, acc, m);
+  }
+}
+
+// --------------------------------------------------------------------------------------- host
+int elem_size(int dtype) { return dtype == REGCN_F32 ? 4 : 2; }
+
+struct GradWs {
+  int2* runs;
+  uint32_t* key[2];
+  int32_t* val[2];
+  uint32_t* hist;
+  float *part, *part2;
+  int64_t dp, bytes;
+};
+
+// The workspace's parts (ws null: sizes only).  16-byte pieces of 2-byte elements are the widest,
+// so the partial rows are rounded up to 8 columns.
+GradWs grad_ws(int64_t n, int64_t V, int d, void* ws) {
+  GradWs w{};
+  char* p = (char*)ws;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    char* q = p ? p + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  w.dp = ((int64_t)d + 7) / 8 * 8;
+  w.runs = (int2*)take(V * 8);
+  for (int k = 0; k < 2; ++k) {
+    const bool need = k == 0 || n > RANK_MAX;
+    w.key[k] = (uint32_t*)take(need ? n * 4 : 0);
+    w.val[k] = (int32_t*)take(need ? n * 4 : 0);
+  }
+  w.hist = (uint32_t*)take(n > RANK_MAX ? (int64_t)MAX_TILES * BINS * 4 : 0);
+  w.part = (float*)take(n / BLK * w.dp * 4);
+  w.part2 = (float*)take(n / GRP * w.dp * 4);
+  w.bytes = at;
+  return w;
+}
+
+int check_common(const char* what, const void* idx, int64_t n, int64_t V, int d, int dtype) {
+  if (d <= 0 || n < 0 || V < 0) return set_error(REGCN_EINVAL, "%s: bad size (n=%lld V=%lld d=%d)", what, (long long)n, (long long)V, d);
+  if (n > 0x7fffffff - 1024 || V >= 0x7fffffff) return set_error(REGCN_ENOTSUP, "%s: n and V below 2^31", what);
+  if (dtype < REGCN_F32 || dtype > REGCN_F16) return set_error(REGCN_EINVAL, "%s: bad element type %d", what, dtype);
+  if (n > 0 && !idx) return set_error(REGCN_EINVAL, "%s: null index", what);
+  return 0;
+}
+
+template <typename T>
+int launch_lookup(const void* table, int64_t ld, const Tokens& t, int d, float scale, void* out, hipStream_t st) {
+  const int64_t total = t.n * ((d + Piece<T>::VE - 1) / Piece<T>::VE);
+  const int64_t wgs = (total + ROW_THR - 1) / ROW_THR;
+  k_lookup<T><<<(int)std::min<int64_t>(wgs, 1 << 20), ROW_THR, 0, st>>>((const T*)table, ld, t, d, scale, (T*)out);
+  return check_launch("embedding lookup");
+}
+
+template <typename T>
+int launch_grad(const void* g, const Tokens& t, int d, float scale, void* out, const GradWs& w, hipStream_t st) {
+  constexpr int VE = Piece<T>::VE;
+  const int64_t n = t.n, V = t.V;
+  const int clear_wgs = (int)std::min<int64_t>((V + 4 * SORT_THR - 1) / (4 * SORT_THR), 1024);
+  int side = 0;  // which of the key / val pairs holds the sorted tokens
+  if (n <= RANK_MAX) {
+    const int wgs = std::max((int)((n + WAVE - 1) / WAVE), clear_wgs);
+    if (wgs > 0)
+      k_rank<<<wgs, SORT_THR, 0, st>>>(t, w.val[0], w.key[0], w.runs);
+  } else {
+    int bits = 0;
+    while (V >> bits) ++bits;  // the key V itself included
+    const int passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
+    int64_t tile = (n + MAX_TILES - 1) / MAX_TILES;
+    tile = std::max<int64_t>((tile + SORT_THR - 1) / SORT_THR * SORT_THR, 2 * SORT_THR);
+    const int tiles = (int)((n + tile - 1) / tile);
+    for (int p = 0; p < passes; ++p) {
+      const uint32_t* ki = p ? w.key[side] : nullptr;
+      const int32_t* vi = p ? w.val[side] : nullptr;
+      const int to = p ? 1 - side : 0;
+      k_hist<<<tiles, SORT_THR, 0, st>>>(t, ki, p * RADIX_BITS, tile, w.hist, p ? nullptr : w.runs);
+      k_scatter<<<tiles, SORT_THR, 0, st>>>(t, ki, vi, p * RADIX_BITS, tile, w.hist, w.key[to], w.val[to]);
+      side = to;
+    }
+  }
+  if (int rc = check_launch("embedding gradient sort")) return rc;
+  const uint32_t* skey = w.key[side];
+  const int32_t* perm = w.val[side];
+  if (n > 0)
+    k_block_sums<T><<<(int)((n + BLK - 1) / BLK), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, w.runs,
+                                                                    w.part);
+  if (n >= GRP) k_group_sums<VE><<<(int)(n / GRP), ROW_THR, 0, st>>>(skey, V, w.dp, w.part, w.part2);
+  const int C = (int)((w.dp + VE - 1) / VE);
+  const int rows = std::max(1, 2048 / C);
+  k_row_grads<T><<<(int)((V + rows - 1) / rows), ROW_THR, 0, st>>>((const T*)g, perm, w.runs, w.part, w.part2, V, d,
+                                                                  w.dp, rows, scale, (T*)out);
+  return check_launch("embedding gradient");
+}
+
+}  // namespace
+
+int64_t embedding_grad_ws_bytes(int64_t n, int64_t V, int d) {
+  if (n < 0 || V < 0 || d <= 0) return 0;
+  return grad_ws(n, V, d, nullptr).bytes;
+}
+
+int embedding(const void* table, int64_t ld, const void* idx, int wide, int64_t n, int64_t V, int d, int dtype, float scale,
+              void* out, hipStream_t st) {
+  if (int rc = check_common("embedding", idx, n, V, d, dtype)) return rc;
+  if (n == 0) return 0;
+  if ((V > 0 && !table) || !out) return set_error(REGCN_EINVAL, "embedding: null table or output");
+  if (V > 1 && ld < d) return set_error(REGCN_EINVAL, "embedding: row stride %lld below d=%d", (long long)ld, d);
+  const Tokens t{idx, wide != 0, n, V, -1};
+  if (dtype == REGCN_F32) return launch_lookup<float>(table, ld, t, d, scale, out, st);
+  if (dtype == REGCN_BF16) return launch_lookup<__bf16>(table, ld, t, d, scale, out, st);
+  return launch_lookup<_Float16>(table, ld, t, d, scale, out, st);
+}
+
+int embedding_grad(const void* g, const void* idx, int wide, int64_t n, int64_t V, int d, int64_t pad, int dtype,
+                   float scale, void* out, void* ws, size_t ws_bytes, hipStream_t st) {
+  if (int rc = check_common("embedding gradient", idx, n, V, d, dtype)) return rc;
+  if (V == 0) return 0;
+  if ((n > 0 && !g) || !out) return set_error(REGCN_EINVAL, "embedding gradient: null gradient or output");
+  const GradWs w = grad_ws(n, V, d, ws);
+  if (!ws || ws_bytes < (size_t)w.bytes)
+    return set_error(REGCN_EINVAL, "embedding gradient: workspace of %zu bytes, needs %lld", ws_bytes, (long long)w.bytes);
+  const Tokens t{idx, wide != 0, n, V, pad < 0 ? -1 : pad};
+  if (dtype == REGCN_F32) return launch_grad<float>(g, t, d, scale, out, w, st);
+  if (dtype == REGCN_BF16) return launch_grad<__bf16>(g, t, d, scale, out, w, st);
+  return launch_grad<_Float16>(g, t, d, scale, out, w, st);
+}
+
+}  // namespace regcn

@@ -353,4 +353,11 @@ int rank_fused(ScoreArgs& a, int accumulate, int* counts, hipStream_t st);
 int rank(const float* S, int B, int N, const int* target, const float* ts, const int* filt_ptr, const int* filt_idx,
          int add, int* rank_raw, int* rank_filt, hipStream_t st);
 
+// lookup.hip
+int embedding(const void* table, int64_t ld, const void* idx, int wide, int64_t n, int64_t V, int d, int dtype, float scale,
+              void* out, hipStream_t st);
+int64_t embedding_grad_ws_bytes(int64_t n, int64_t V, int d);
+int embedding_grad(const void* g, const void* idx, int wide, int64_t n, int64_t V, int d, int64_t pad, int dtype,
+                   float scale, void* out, void* ws, size_t ws_bytes, hipStream_t st);
+
 }  // namespace regcn

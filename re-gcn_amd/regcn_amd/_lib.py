@@ -8,6 +8,7 @@ torch is imported before the library so that libregcn_hip.so binds to the same
 libamdhip64 instance (same soname) that torch already loaded: one HIP runtime, one
 set of streams.
 """
+import contextlib
 import ctypes
 import os
 
@@ -105,7 +106,12 @@ _SIGS = {
     "regcn_lorentz_aggregate_bwd_f32": [P, _c_int, _c_f, P],
     "regcn_hyp_ce_lse_f32": [P, P, P, P, P, P, _c_int, _c_int, _c_int, _c_f, _c_int, P, P, P, P],
     "regcn_hyp_ce_bwd_f32": [P, P, P, P, P, P, P, P, _c_int, _c_int, _c_int, _c_f, _c_int, P, P, P, P],
+    "regcn_embedding": [P, _c_i64, P, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_f, P, P],
+    "regcn_embedding_grad_workspace_bytes": [_c_i64, _c_i64, _c_int],
+    "regcn_embedding_grad": [P, P, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_f, P, P, _c_sz, P],
 }
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # REGCN_F32, REGCN_BF16, REGCN_F16
 
 SCORE_DIST, SCORE_RAW_SCALE = 1, 2
 _RESTYPE = {"regcn_last_error_string": ctypes.c_char_p, "regcn_hyp_ce_workspace_bytes": _c_sz,
@@ -114,7 +120,7 @@ _RESTYPE = {"regcn_last_error_string": ctypes.c_char_p, "regcn_hyp_ce_workspace_
             "regcn_row_src_order_workspace_bytes": _c_sz, "regcn_item_src_order_workspace_bytes": _c_sz,
             "regcn_packed_weight_kp_floats": _c_sz,
             "regcn_packed_weight_floats": _c_sz, "regcn_packed_linear_floats": _c_sz,
-            "regcn_packed_k4_floats": _c_sz}
+            "regcn_packed_k4_floats": _c_sz, "regcn_embedding_grad_workspace_bytes": _c_i64}
 
 _lib = None
 
@@ -291,6 +297,13 @@ def publish():
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on(device):
+    """Context that makes `device` the current one (its stream, its allocations); free when it is already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def addr(t, dtype=torch.float32, what="tensor"):

@@ -687,3 +687,78 @@ def batch_norm(bn, x):
     if bn.training or torch.is_grad_enabled() or not x.is_cuda:
         return bn(x)
     return torch.native_batch_norm(x, bn.weight, bn.bias, bn.running_mean, bn.running_var, False, 0.0, bn.eps)[0]
+
+
+# ------------------------------------------------------------------ embedding rows
+def _embedding_rows(table, idx, scale):
+    out = torch.empty(idx.shape + (table.shape[1],), device=table.device, dtype=table.dtype)
+    if out.numel():
+        with _lib.on(table.device):
+            _lib.call("regcn_embedding", table.data_ptr(), table.stride(0), idx.data_ptr(), int(idx.dtype == torch.int64),
+                      idx.numel(), table.shape[0], table.shape[1], _lib.DTYPES[table.dtype], scale, out.data_ptr(),
+                      _lib.stream())
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, idx, scale, pad):
+        ctx.save_for_backward(idx)
+        ctx.V, ctx.d, ctx.dtype, ctx.scale, ctx.pad = table.shape[0], table.shape[1], table.dtype, scale, pad
+        return _embedding_rows(table, idx, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (idx,) = ctx.saved_tensors
+        V, d, n = ctx.V, ctx.d, idx.numel()
+        g = g.contiguous()
+        grad = torch.empty(V, d, device=g.device, dtype=ctx.dtype)
+        if grad.numel():
+            size = _lib.lib().regcn_embedding_grad_workspace_bytes(n, V, d)
+            ws = torch.empty(size, device=g.device, dtype=torch.uint8)
+            with _lib.on(g.device):
+                _lib.call("regcn_embedding_grad", g.data_ptr(), idx.data_ptr(), int(idx.dtype == torch.int64), n, V, d,
+                          ctx.pad, _lib.DTYPES[ctx.dtype], ctx.scale, grad.data_ptr(), ws.data_ptr(), size,
+                          _lib.stream())
+        return grad, None, None, None
+
+
+def embedding(table, idx, scale=1.0, padding_idx=None):
+    """scale * table[idx]: rows of a (V x d) fp32, bf16 or fp16 table for int32 / int64 indices of any
+    shape, in one launch (regcn_embedding).  The gradient is dense, in the table's type: each row's
+    tokens are summed in fp32 in a fixed order over tokens sorted by index, without atomics
+    (regcn_embedding_grad), so it has the same bits on every call; rows of `padding_idx` (counted from
+    the end when negative) take no gradient.  An index outside [0, V) reads nothing: its output row is
+    NaN, and no gradient row takes it (checking it would wait for the device).  Rows may be strided;
+    a table whose columns are not adjacent is copied.  Differentiable once, with respect to `table`.
+
+    Inside a HIP-graph capture the usual rule of captured backward passes holds: no autograd graph of
+    an eager pass over the same leaves may be alive."""
+    if not isinstance(table, torch.Tensor) or not isinstance(idx, torch.Tensor):
+        raise TypeError("embedding takes tensors (table: %s, idx: %s)" % (type(table).__name__, type(idx).__name__))
+    if table.dim() != 2:
+        raise ValueError("table must be V x d (got %s)" % (tuple(table.shape),))
+    if table.dtype not in _lib.DTYPES:
+        raise TypeError("table must be float32, bfloat16 or float16 (got %s)" % table.dtype)
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError("idx must be int64 or int32 (got %s)" % idx.dtype)
+    if not table.is_cuda or idx.device != table.device:
+        raise ValueError("table and idx must live on one HIP device (got %s, %s); the HIP path has no CPU fallback"
+                         % (table.device, idx.device))
+    V = table.shape[0]
+    pad = -1
+    if padding_idx is not None:
+        pad = int(padding_idx)
+        if not -V <= pad < V:
+            raise ValueError("padding_idx %d is outside the table's %d rows" % (pad, V))
+        pad %= V
+    if V >= 2 ** 31 - 1 or idx.numel() > 2 ** 31 - 1025:
+        raise ValueError("embedding takes fewer than 2^31 rows and tokens (got %d, %d)" % (V, idx.numel()))
+    scale = float(scale)
+    idx = idx.contiguous()
+    if table.shape[1] > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    if needs_grad(table):
+        return _Embedding.apply(table, idx, scale, pad)
+    return _embedding_rows(table.detach(), idx, scale)
