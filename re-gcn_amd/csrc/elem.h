@@ -35,14 +35,18 @@ __device__ __forceinline__ void load_piece(float (&o)[Piece<T>::VE], const T* __
   }
 }
 
+// p[0..m) = o; `stream`: past the caches (an output larger than they hold).
 template <typename T>
-__device__ __forceinline__ void store_piece(T* __restrict__ p, const float (&o)[Piece<T>::VE], int m) {
+__device__ __forceinline__ void store_piece(T* __restrict__ p, const float (&o)[Piece<T>::VE], int m, bool stream = false) {
   constexpr int VE = Piece<T>::VE;
   if (m >= VE) {
     typename Piece<T>::vec v;
 #pragma unroll
     for (int e = 0; e < VE; ++e) v[e] = from_f32<T>(o[e]);
-    *reinterpret_cast<typename Piece<T>::uvec*>(p) = v;
+    if (stream)
+      __builtin_nontemporal_store((typename Piece<T>::uvec)v, reinterpret_cast<typename Piece<T>::uvec*>(p));
+    else
+      *reinterpret_cast<typename Piece<T>::uvec*>(p) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < VE; ++e)

@@ -13,22 +13,28 @@
 // sorted positions, then sums the runs in a fixed order: no atomics, the same bits on every call.
 //   * up to RANK_MAX tokens one launch ranks each token by counting the keys before it;
 //   * more take least-significant-digit radix passes of 10 bits (two launches a pass).
-// A run of any length is summed in three levels: whole 64-token blocks inside a run are summed by
-// k_block_sums, whole groups of 64 such blocks by k_group_sums, and the row's thread adds its ends
-// to those.  Sums are fp32; a 16-bit type is rounded once, at the store.
+// A run of any length is summed over a tree of fan 16 on the sorted positions (k_partials: nodes whose
+// tokens all belong to one row); the row's thread adds the at most 15 tokens or nodes at each end of
+// each level, so no chain of dependent loads grows with the run.  Sums are fp32; a 16-bit type is
+// rounded once, at the store.
 #include "elem.h"
 #include "regcn_internal.h"
 
 namespace regcn {
 namespace {
 
-constexpr int RANK_MAX = 16384;    // tokens ranked by counting (their keys in 64 KB of LDS)
-constexpr int BLK = 64;            // sorted positions of a block
-constexpr int GRP = BLK * BLK;     // ... of a group of blocks
+constexpr int RANK_MAX = 8192;     // tokens ranked by counting (their keys in 32 KB of LDS)
+constexpr int FAN = 16, LEVELS = 5;  // the tree of partial sums: 16, 256, 4096, 65536 tokens a node
 constexpr int RADIX_BITS = 10, BINS = 1 << RADIX_BITS;
 constexpr int MAX_TILES = 256;     // radix tiles (a workgroup each)
 constexpr int SORT_THR = 1024, SORT_WAVES = SORT_THR / WAVE;
 constexpr int ROW_THR = 256;
+// Outputs above half of the card's L2s (8 x 4 MB) are stored past them: nothing of them is left there for
+// a reader anyway, and the rows being read stay (a 33 MB lookup: 15.5 -> 10.2 us, a 210 MB one 82 -> 68 us,
+// a 268 MB gradient 75 -> 59 us).  Smaller ones stay cached for the kernel that reads them next.
+constexpr int64_t STREAM_BYTES = 16 << 20;
+constexpr int MAX_ROWS = 512;      // rows a workgroup of k_row_grads
+constexpr int SLICE = 16;          // 16-byte pieces of the columns a workgroup of k_partials takes
 
 struct Tokens {
   const void* idx;
@@ -45,7 +51,7 @@ __device__ __forceinline__ uint32_t token_key(const Tokens& t, int64_t i) {
 // ------------------------------------------------------------------------------------ forward
 template <typename T>
 __global__ __launch_bounds__(ROW_THR) void k_lookup(const T* __restrict__ table, int64_t ld, Tokens t, int d,
-                                                    float scale, T* __restrict__ out) {
+                                                    float scale, bool stream_out, T* __restrict__ out) {
   constexpr int VE = Piece<T>::VE;
   const int C = (d + VE - 1) / VE;
   const int64_t total = t.n * C;
@@ -63,7 +69,7 @@ __global__ __launch_bounds__(ROW_THR) void k_lookup(const T* __restrict__ table,
     }
 #pragma unroll
     for (int e = 0; e < VE; ++e) x[e] *= scale;
-    store_piece<T>(out + i * d + c0, x, m);
+    store_piece<T>(out + i * d + c0, x, m, stream_out);
   }
 }
 
@@ -96,11 +102,17 @@ __global__ __launch_bounds__(SORT_THR) void k_rank(Tokens t, int32_t* __restrict
   // keys of the lower positions count when <= k, those of the higher ones when < k; the 64
   // positions around i0 are told apart one by one
   const int lo = min(j1, i0), hi = max(j0, i0 + WAVE);
+#pragma unroll 8
   for (int j = j0; j < lo; j += 4) {
     const uint4 q = *(const uint4*)(keys + j);
     cnt += (q.x <= k) + (q.y <= k) + (q.z <= k) + (q.w <= k);
   }
-  for (int j = max(j0, i0); j < min(j1, i0 + WAVE); ++j) cnt += keys[j] < k || (keys[j] == k && j < i);
+#pragma unroll 4
+  for (int j = max(j0, i0); j < min(j1, i0 + WAVE); j += 4) {
+    const uint4 q = *(const uint4*)(keys + j);
+    cnt += (q.x < k + (j < i)) + (q.y < k + (j + 1 < i)) + (q.z < k + (j + 2 < i)) + (q.w < k + (j + 3 < i));
+  }
+#pragma unroll 8
   for (int j = hi; j < j1; j += 4) {
     const uint4 q = *(const uint4*)(keys + j);
     cnt += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
@@ -146,6 +158,7 @@ __global__ __launch_bounds__(SORT_THR) void k_scatter(Tokens t, const uint32_t* 
   const int tiles = gridDim.x, me = blockIdx.x;
   static_assert(BINS == SORT_THR, "a thread per bin");
   uint32_t before = 0, total = 0;
+#pragma unroll 32
   for (int s = 0; s < tiles; ++s) {
     const uint32_t c = hist[(int64_t)s * BINS + tid];
     before += s < me ? c : 0;
@@ -200,40 +213,41 @@ __global__ __launch_bounds__(SORT_THR) void k_scatter(Tokens t, const uint32_t* 
 }
 
 // --------------------------------------------------------------------------------------- sums
-// acc += rows src[0..cnt) of width-d pieces; src[j] = base + row(j) * d.
+// acc += the row pieces row(0) .. row(cnt - 1) in order, up to eight loads in flight.
 template <typename T, typename Row>
-__device__ __forceinline__ void add_rows(float (&acc)[Piece<T>::VE], const T* __restrict__ base, int64_t d, int c0, int m,
-                                         int cnt, Row row) {
-  constexpr int VE = Piece<T>::VE, U = 4;
+__device__ __forceinline__ void add_rows(float (&acc)[Piece<T>::VE], int m, int cnt, Row row) {
+  constexpr int VE = Piece<T>::VE, U = 8;
   int j = 0;
   for (; j + U <= cnt; j += U) {
     float x[U][VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_piece<T>(x[u], base + row(j + u) * d + c0, m);
+    for (int u = 0; u < U; ++u) load_piece<T>(x[u], row(j + u), m);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < VE; ++e) acc[e] += x[u][e];
   }
-  for (; j < cnt; ++j) {
-    float x[VE];
-    load_piece<T>(x, base + row(j) * d + c0, m);
+  for (; j < cnt; j += 2) {
+    float x[2][VE];
+    load_piece<T>(x[0], row(j), m);
+    load_piece<T>(x[1], row(min(j + 1, cnt - 1)), m);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[e] += x[e];
+    for (int e = 0; e < VE; ++e) {
+      acc[e] += x[0][e];
+      acc[e] = j + 1 < cnt ? acc[e] + x[1][e] : acc[e];
+    }
   }
 }
 
-// A partial row piece (VE floats of the fp32 partial sums).
+// The same over cnt fp32 partial rows dp apart.
 template <int VE>
-__device__ __forceinline__ void add_partials(float (&acc)[VE], const float* __restrict__ part, int64_t dp, int c0, int cnt) {
-  for (int j = 0; j < cnt; ++j) {
-    const f4* q = reinterpret_cast<const f4*>(part + j * dp + c0);
+__device__ __forceinline__ void add_partials(float (&acc)[VE], const float* __restrict__ part, int64_t dp, int cnt) {
 #pragma unroll
-    for (int h = 0; h < VE / 4; ++h) {
-      const f4 v = q[h];
+  for (int h = 0; h < VE / 4; ++h) {
+    float a[4] = {acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
+    add_rows<float>(a, 4, cnt, [&](int j) { return part + j * dp + 4 * h; });
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[4 * h + e] += v[e];
-    }
+    for (int e = 0; e < 4; ++e) acc[4 * h + e] = a[e];
   }
 }
 
@@ -244,89 +258,107 @@ __device__ __forceinline__ void store_partial(float* __restrict__ part, const fl
   for (int h = 0; h < VE / 4; ++h) q[h] = f4{acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
 }
 
-// Per 64 sorted positions: the ends of the runs that lie in them, and their sum where all 64
-// belong to one row.  dp: the partial rows' width (d rounded up to whole pieces).
-template <typename T>
-__global__ __launch_bounds__(ROW_THR) void k_block_sums(const T* __restrict__ g, const int32_t* __restrict__ perm,
-                                                        const uint32_t* __restrict__ skey, int64_t n, int64_t V, int d,
-                                                        int64_t dp, int2* __restrict__ runs, float* __restrict__ part) {
+// Partial sums: level 0 is the sorted tokens; a node of level l + 1 is the sum of FAN nodes of level l
+// and exists where all its tokens belong to one row.
+struct Levels {
+  float* part[LEVELS];  // [1..]: nodes of dp floats
+};
+
+// Two levels in one launch, a workgroup per FAN * FAN nodes of level `lo`: the sums of FAN nodes each
+// (level lo + 1), then, where the whole workgroup's tokens belong to one row, of those (lo + 2).
+// Level 0 also writes the ends of the runs that lie in its tokens.
+template <typename T, int LO>
+__global__ __launch_bounds__(ROW_THR) void k_partials(const T* __restrict__ g, const int32_t* __restrict__ perm,
+                                                      const uint32_t* __restrict__ skey, int64_t n, int64_t V, int d,
+                                                      int64_t dp, int2* __restrict__ runs, Levels lv) {
   constexpr int VE = Piece<T>::VE;
-  const int64_t p0 = (int64_t)blockIdx.x * BLK;
-  if (threadIdx.x < BLK) {
+  constexpr int64_t NODE = LO == 0 ? FAN : (int64_t)FAN * FAN * FAN;  // tokens of a node of level LO + 1
+  const int64_t p0 = (int64_t)blockIdx.x * NODE * FAN;
+  __shared__ int32_t tok[LO == 0 ? FAN * FAN : 1];
+  __shared__ int full[FAN];
+  if (LO == 0) {  // (every column slice writes the same runs)
+    static_assert(LO != 0 || ROW_THR == FAN * FAN, "a thread per token");
     const int64_t p = p0 + threadIdx.x;
     if (p < n) {
       const uint32_t k = skey[p];
+      tok[threadIdx.x] = perm[p];
       if (k < V) {
         if (p == 0 || skey[p - 1] != k) runs[k].x = (int)p;
         if (p == n - 1 || skey[p + 1] != k) runs[k].y = (int)p + 1;
       }
     }
   }
-  if (p0 + BLK > n) return;
-  const uint32_t k0 = skey[p0];
-  if (k0 >= V || skey[p0 + BLK - 1] != k0) return;
-  const int C = (int)(dp / VE);
-  for (int c = threadIdx.x; c < C; c += ROW_THR) {
+  if (threadIdx.x < FAN) {
+    const int64_t q = p0 + threadIdx.x * NODE;
+    full[threadIdx.x] = q + NODE <= n && skey[q] < V && skey[q] == skey[q + NODE - 1];
+  }
+  __syncthreads();
+  const int per = ((int)(dp / VE) + gridDim.y - 1) / gridDim.y;  // this workgroup's pieces of the columns
+  const int slice = blockIdx.y * per;
+  const int C = min((int)(dp / VE) - slice, per);
+  const int64_t node0 = (int64_t)blockIdx.x * FAN;
+  const int b = threadIdx.x / SLICE, c0 = (slice + threadIdx.x % SLICE) * VE;
+  static_assert(FAN * SLICE == ROW_THR, "a thread per node and piece");
+  if (full[b] && (int)(threadIdx.x % SLICE) < C) {
     float acc[VE] = {};
-    add_rows<T>(acc, g, d, c * VE, d - c * VE, BLK, [&](int j) { return (int64_t)perm[p0 + j]; });
-    store_partial<VE>(part + (int64_t)blockIdx.x * dp + c * VE, acc);
+    if (LO == 0)
+      add_rows<T>(acc, d - c0, FAN, [&](int j) { return g + (int64_t)tok[b * FAN + j] * d + c0; });
+    else
+      add_partials<VE>(acc, lv.part[LO] + (node0 + b) * FAN * dp + c0, dp, FAN);
+    store_partial<VE>(lv.part[LO + 1] + (node0 + b) * dp + c0, acc);
+  }
+  if (p0 + NODE * FAN > n || skey[p0] >= V || skey[p0] != skey[p0 + NODE * FAN - 1]) return;
+  __syncthreads();  // all FAN nodes of level LO + 1 exist and are written
+  if ((int)threadIdx.x < C) {
+    float acc[VE] = {};
+    add_partials<VE>(acc, lv.part[LO + 1] + node0 * dp + c0, dp, FAN);
+    store_partial<VE>(lv.part[LO + 2] + (int64_t)blockIdx.x * dp + c0, acc);
   }
 }
 
-// Per 4096 sorted positions of one row: the sum of its 64 block sums.
-template <int VE>
-__global__ __launch_bounds__(ROW_THR) void k_group_sums(const uint32_t* __restrict__ skey, int64_t V, int64_t dp,
-                                                        const float* __restrict__ part, float* __restrict__ part2) {
-  const int64_t p0 = (int64_t)blockIdx.x * GRP;
-  const uint32_t k0 = skey[p0];
-  if (k0 >= V || skey[p0 + GRP - 1] != k0) return;
-  const int C = (int)(dp / VE);
-  for (int c = threadIdx.x; c < C; c += ROW_THR) {
-    float acc[VE] = {};
-    add_partials<VE>(acc, part + (int64_t)blockIdx.x * BLK * dp, dp, c * VE, BLK);
-    store_partial<VE>(part2 + (int64_t)blockIdx.x * dp + c * VE, acc);
-  }
-}
-
-// Every row of dtable, once: s * (tokens before the first whole block + block sums + group sums +
-// block sums + tokens after the last whole block), zero for a row without tokens.
+// Every row of dtable, once: s times the sum of its run of sorted tokens, taken as the run's ends at
+// each level and the nodes between them; zero for a row without tokens.
 template <typename T>
 __global__ __launch_bounds__(ROW_THR) void k_row_grads(const T* __restrict__ g, const int32_t* __restrict__ perm,
-                                                       const int2* __restrict__ runs, const float* __restrict__ part,
-                                                       const float* __restrict__ part2, int64_t V, int d, int64_t dp,
-                                                       int rows_per_wg, float scale, T* __restrict__ out) {
+                                                       const int2* __restrict__ runs, Levels lv, int64_t V, int d,
+                                                       int64_t dp, int rows_per_wg, float scale, bool stream_out,
+                                                       T* __restrict__ out) {
   constexpr int VE = Piece<T>::VE;
-  const int C = (int)(dp / VE);
+  const int C = (d + VE - 1) / VE;
   const int64_t v0 = (int64_t)blockIdx.x * rows_per_wg;
   const int rows = (int)min((int64_t)rows_per_wg, V - v0);
+  __shared__ int2 lrun[MAX_ROWS];  // one wait for all the rows' runs, then stores without loads for empty rows
+  for (int r = threadIdx.x; r < rows; r += ROW_THR) lrun[r] = runs[v0 + r];
+  __syncthreads();
   for (int it = threadIdx.x; it < rows * C; it += ROW_THR) {
     const int r = (int)((uint32_t)it / (uint32_t)C);
     const int c0 = (it - r * C) * VE, m = d - c0;
-    const int2 run = runs[v0 + r];
+    const int2 run = lrun[r];
     float acc[VE] = {};
     if (run.x < run.y) {
-      const int b0 = (run.x + BLK - 1) / BLK, b1 = run.y / BLK;  // whole blocks [b0, b1)
-      const auto token = [&](int p) {
-        return [=](int j) { return (int64_t)perm[p + j]; };
-      };
-      if (b0 >= b1) {
-        add_rows<T>(acc, g, d, c0, m, run.y - run.x, token(run.x));
-      } else {
-        add_rows<T>(acc, g, d, c0, m, b0 * BLK - run.x, token(run.x));
-        const int g0 = (b0 + BLK - 1) / BLK, g1 = b1 / BLK;  // whole groups [g0, g1)
-        if (g0 >= g1) {
-          add_partials<VE>(acc, part + b0 * dp, dp, c0, b1 - b0);
-        } else {
-          add_partials<VE>(acc, part + b0 * dp, dp, c0, g0 * BLK - b0);
-          add_partials<VE>(acc, part2 + g0 * dp, dp, c0, g1 - g0);
-          add_partials<VE>(acc, part + (int64_t)g1 * BLK * dp, dp, c0, b1 - g1 * BLK);
+      int lo = run.x, hi = run.y;
+#pragma unroll
+      for (int l = 0; l < LEVELS; ++l) {
+        const auto add = [&](int a, int b) {
+          if (l == 0)
+            add_rows<T>(acc, m, b - a, [&](int j) { return g + (int64_t)perm[a + j] * d + c0; });
+          else
+            add_partials<VE>(acc, lv.part[l] + a * dp + c0, dp, b - a);
+        };
+        const int up = lo / FAN + (lo % FAN != 0), dn = hi / FAN;
+        if (l == LEVELS - 1 || up >= dn) {
+          add(lo, hi);
+          break;
         }
-        add_rows<T>(acc, g, d, c0, m, run.y - b1 * BLK, token(b1 * BLK));
+        add(lo, up * FAN);
+        add(dn * FAN, hi);
+        lo = up;
+        hi = dn;
       }
 #pragma unroll
       for (int e = 0; e < VE; ++e) acc[e] *= scale;
     }
-    store_piece<T>(out + (v0 + r) * d + c0, acc, m);
+    store_piece<T>(out + (v0 + r) * d + c0, acc, m, stream_out);
   }
 }
 
@@ -338,7 +370,7 @@ struct GradWs {
   uint32_t* key[2];
   int32_t* val[2];
   uint32_t* hist;
-  float *part, *part2;
+  Levels lv;
   int64_t dp, bytes;
 };
 
@@ -361,8 +393,7 @@ GradWs grad_ws(int64_t n, int64_t V, int d, void* ws) {
     w.val[k] = (int32_t*)take(need ? n * 4 : 0);
   }
   w.hist = (uint32_t*)take(n > RANK_MAX ? (int64_t)MAX_TILES * BINS * 4 : 0);
-  w.part = (float*)take(n / BLK * w.dp * 4);
-  w.part2 = (float*)take(n / GRP * w.dp * 4);
+  for (int l = 1; l < LEVELS; ++l) w.lv.part[l] = (float*)take((n >> (4 * l)) * w.dp * 4);
   w.bytes = at;
   return w;
 }
@@ -379,7 +410,8 @@ template <typename T>
 int launch_lookup(const void* table, int64_t ld, const Tokens& t, int d, float scale, void* out, hipStream_t st) {
   const int64_t total = t.n * ((d + Piece<T>::VE - 1) / Piece<T>::VE);
   const int64_t wgs = (total + ROW_THR - 1) / ROW_THR;
-  k_lookup<T><<<(int)std::min<int64_t>(wgs, 1 << 20), ROW_THR, 0, st>>>((const T*)table, ld, t, d, scale, (T*)out);
+  k_lookup<T><<<(int)std::min<int64_t>(wgs, 1 << 20), ROW_THR, 0, st>>>((const T*)table, ld, t, d, scale,
+                                                                       t.n * d * (int64_t)sizeof(T) > STREAM_BYTES, (T*)out);
   return check_launch("embedding lookup");
 }
 
@@ -412,14 +444,20 @@ int launch_grad(const void* g, const Tokens& t, int d, float scale, void* out, c
   if (int rc = check_launch("embedding gradient sort")) return rc;
   const uint32_t* skey = w.key[side];
   const int32_t* perm = w.val[side];
+  static_assert(FAN == 16, "levels by shifts of 4");
+  const int slices = (int)((w.dp / VE + SLICE - 1) / SLICE);
   if (n > 0)
-    k_block_sums<T><<<(int)((n + BLK - 1) / BLK), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, w.runs,
-                                                                    w.part);
-  if (n >= GRP) k_group_sums<VE><<<(int)(n / GRP), ROW_THR, 0, st>>>(skey, V, w.dp, w.part, w.part2);
-  const int C = (int)((w.dp + VE - 1) / VE);
-  const int rows = std::max(1, 2048 / C);
-  k_row_grads<T><<<(int)((V + rows - 1) / rows), ROW_THR, 0, st>>>((const T*)g, perm, w.runs, w.part, w.part2, V, d,
-                                                                  w.dp, rows, scale, (T*)out);
+    k_partials<T, 0><<<dim3((int)((n + FAN * FAN - 1) / (FAN * FAN)), slices), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp,
+                                                                                  w.runs, w.lv);
+  if (n >> 12)
+    k_partials<T, 2><<<dim3((int)((n + 65535) / 65536), slices), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, w.runs, w.lv);
+  const int C = (d + VE - 1) / VE;
+  // rows a workgroup: enough for its 256 threads, up to 2048 pieces while that leaves 2048 workgroups
+  const int64_t want = std::min<int64_t>(2048, std::max<int64_t>(ROW_THR, V * C / 2048));
+  const int rows = std::min(MAX_ROWS, std::max(1, (int)(want / C)));
+  k_row_grads<T><<<(int)((V + rows - 1) / rows), ROW_THR, 0, st>>>((const T*)g, perm, w.runs, w.lv, V, d, w.dp, rows,
+                                                                  scale, V * d * (int64_t)sizeof(T) > STREAM_BYTES,
+                                                                  (T*)out);
   return check_launch("embedding gradient");
 }
 

@@ -8,7 +8,6 @@ torch is imported before the library so that libregcn_hip.so binds to the same
 libamdhip64 instance (same soname) that torch already loaded: one HIP runtime, one
 set of streams.
 """
-import contextlib
 import ctypes
 import os
 
@@ -299,11 +298,17 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def on(device):
-    """Context that makes `device` the current one (its stream, its allocations); free when it is already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def launch(name, device, *args):
+    """`call` of an entry whose last argument is the stream, on `device`'s current stream (which need not
+    be the current device).  The lean form for small launches: no ctypes objects are built."""
+    fn = getattr(_lib or lib(), name)
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != 0 or EVENT_TRACE is not None:
+        check(rc, name)
 
 
 def addr(t, dtype=torch.float32, what="tensor"):

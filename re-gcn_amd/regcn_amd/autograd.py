@@ -691,37 +691,58 @@ def batch_norm(bn, x):
 
 # ------------------------------------------------------------------ embedding rows
 def _embedding_rows(table, idx, scale):
-    out = torch.empty(idx.shape + (table.shape[1],), device=table.device, dtype=table.dtype)
-    if out.numel():
-        with _lib.on(table.device):
-            _lib.call("regcn_embedding", table.data_ptr(), table.stride(0), idx.data_ptr(), int(idx.dtype == torch.int64),
-                      idx.numel(), table.shape[0], table.shape[1], _lib.DTYPES[table.dtype], scale, out.data_ptr(),
-                      _lib.stream())
+    V, d = table.shape
+    out = torch.empty(idx.shape + (d,), device=table.device, dtype=table.dtype)
+    n = idx.numel()
+    if n and d:
+        _lib.launch("regcn_embedding", table.device, table.data_ptr(), table.stride(0), idx.data_ptr(),
+                    idx.dtype == torch.int64, n, V, d, _lib.DTYPES[table.dtype], scale, out.data_ptr())
     return out
+
+
+def _embedding_sums(g, idx, V, scale, pad):
+    d, n = g.shape[-1], idx.numel()
+    g = g.contiguous()
+    grad = torch.empty(V, d, device=g.device, dtype=g.dtype)
+    if V and d:
+        size = _lib.lib().regcn_embedding_grad_workspace_bytes(n, V, d)
+        ws = torch.empty(size, device=g.device, dtype=torch.uint8)
+        _lib.launch("regcn_embedding_grad", g.device, g.data_ptr(), idx.data_ptr(), idx.dtype == torch.int64, n, V, d,
+                    pad, _lib.DTYPES[g.dtype], scale, grad.data_ptr(), ws.data_ptr(), size)
+    return grad
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, idx, scale, pad):
         ctx.save_for_backward(idx)
-        ctx.V, ctx.d, ctx.dtype, ctx.scale, ctx.pad = table.shape[0], table.shape[1], table.dtype, scale, pad
+        ctx.V, ctx.scale, ctx.pad = table.shape[0], scale, pad
         return _embedding_rows(table, idx, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         (idx,) = ctx.saved_tensors
-        V, d, n = ctx.V, ctx.d, idx.numel()
-        g = g.contiguous()
-        grad = torch.empty(V, d, device=g.device, dtype=ctx.dtype)
-        if grad.numel():
-            size = _lib.lib().regcn_embedding_grad_workspace_bytes(n, V, d)
-            ws = torch.empty(size, device=g.device, dtype=torch.uint8)
-            with _lib.on(g.device):
-                _lib.call("regcn_embedding_grad", g.data_ptr(), idx.data_ptr(), int(idx.dtype == torch.int64), n, V, d,
-                          ctx.pad, _lib.DTYPES[ctx.dtype], ctx.scale, grad.data_ptr(), ws.data_ptr(), size,
-                          _lib.stream())
-        return grad, None, None, None
+        if torch.is_grad_enabled():  # create_graph: the gradient is differentiable in g
+            return _EmbeddingSums.apply(g, idx, ctx.V, ctx.scale, ctx.pad), None, None, None
+        return _embedding_sums(g, idx, ctx.V, ctx.scale, ctx.pad), None, None, None
+
+
+class _EmbeddingSums(torch.autograd.Function):
+    """The gradient of a lookup as a function of g: linear, its own gradient a lookup without the
+    rows of tokens that it leaves out."""
+
+    @staticmethod
+    def forward(ctx, g, idx, V, scale, pad):
+        ctx.save_for_backward(idx)
+        ctx.V, ctx.scale, ctx.pad = V, scale, pad
+        return _embedding_sums(g, idx, V, scale, pad)
+
+    @staticmethod
+    def backward(ctx, gg):
+        (idx,) = ctx.saved_tensors
+        out = embedding(gg, idx, ctx.scale)
+        left = (idx < 0) | (idx >= ctx.V) | (idx == ctx.pad)
+        return out.masked_fill(left.unsqueeze(-1), 0.0), None, None, None, None
 
 
 def embedding(table, idx, scale=1.0, padding_idx=None):
@@ -731,7 +752,7 @@ def embedding(table, idx, scale=1.0, padding_idx=None):
     (regcn_embedding_grad), so it has the same bits on every call; rows of `padding_idx` (counted from
     the end when negative) take no gradient.  An index outside [0, V) reads nothing: its output row is
     NaN, and no gradient row takes it (checking it would wait for the device).  Rows may be strided;
-    a table whose columns are not adjacent is copied.  Differentiable once, with respect to `table`.
+    a table whose columns are not adjacent is copied.
 
     Inside a HIP-graph capture the usual rule of captured backward passes holds: no autograd graph of
     an eager pass over the same leaves may be alive."""

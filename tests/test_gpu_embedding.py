@@ -169,6 +169,21 @@ def test_gradient_against_differences():
             assert abs(float(diff) - float(t.grad[v, j])) <= 9 * (h * h / 6 + 4 * 2.0 ** -23) + 1e-11 / h
 
 
+def test_gradient_of_the_gradient():
+    """grad(table) is linear in the output's gradient g: with f = sum(grad^2) / 2, df/dg_i = s grad[idx_i],
+    0 for a token left out.  Each side is one fp32 product of the same fp32 row."""
+    V, d = 11, 6
+    table = torch.randn(V, d, device=DEV, requires_grad=True)
+    idx = torch.tensor([1, 4, 4, 0, 10, 10, 10, V, 3], device=DEV)
+    g = torch.randn(9, d, device=DEV, requires_grad=True)
+    out = A.embedding(table, idx, 0.5, padding_idx=3)
+    grad, = torch.autograd.grad(out, table, g, create_graph=True)
+    dg, = torch.autograd.grad((grad * grad).sum() * 0.5, g)
+    keep = ((idx < V) & (idx != 3)).unsqueeze(1)
+    want = torch.where(keep, 0.5 * grad.detach()[idx.clamp(max=V - 1)], torch.zeros((), device=DEV))
+    assert torch.equal(dg, want)
+
+
 def test_second_stream_and_broadcast_gradient():
     table = torch.randn(300, 64, device=DEV, requires_grad=True)
     idx = tokens(300, 5000, 2, "hubs").to(DEV)
