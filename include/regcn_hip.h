@@ -854,6 +854,23 @@ int64_t regcn_embedding_grad_workspace_bytes(int64_t n, int64_t V, int32_t d);
 int regcn_embedding_grad(const void* grad, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d, int64_t pad,
                          int32_t dtype, float scale, void* out, void* workspace, size_t ws_bytes, void* stream);
 
+/* ---- Orthogonalising matrices ----------------------------------------------------------- */
+/* A contiguous rows x cols matrix of `dtype` and where its result goes (the same shape and type; out
+ * may be x). */
+typedef struct regcn_matrix {
+  const void* x;
+  void* out;
+  int64_t rows, cols;
+  int32_t dtype;
+} regcn_matrix;
+/* Newton-Schulz iteration of each matrix on its shorter side: X = G / (|G|_F + eps), then `steps` times
+ * A = X X^T, X = a X + (b A + c A A) X, as exact as fp32 products, one rounding to the result's type.
+ * a, b, c must keep the iteration of a singular value, s <- a s + b s^3 + c s^5 from [0, 1], within
+ * [-4, 4]: the operands are held in fp16 halves.  `mats` is host memory and read before the call returns. */
+int64_t regcn_orthogonalize_workspace_bytes(const regcn_matrix* mats, int32_t n_mats);
+int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps, float a, float b, float c, float eps,
+                        void* workspace, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -793,4 +793,12 @@ int regcn_embedding_grad(const void* grad, const void* idx, int32_t idx_wide, in
   return embedding_grad(grad, idx, idx_wide, n, V, d, pad, dtype, scale, out, workspace, ws_bytes, ST(s));
 }
 
+int64_t regcn_orthogonalize_workspace_bytes(const regcn_matrix* mats, int32_t n_mats) {
+  return orthogonalize_ws_bytes(mats, n_mats);
+}
+int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps, float a, float b, float c, float eps,
+                        void* workspace, size_t ws_bytes, void* s) {
+  return orthogonalize(mats, n_mats, steps, a, b, c, eps, workspace, ws_bytes, ST(s));
+}
+
 }  // extern "C"

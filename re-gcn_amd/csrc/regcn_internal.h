@@ -360,4 +360,9 @@ int64_t embedding_grad_ws_bytes(int64_t n, int64_t V, int d);
 int embedding_grad(const void* g, const void* idx, int wide, int64_t n, int64_t V, int d, int64_t pad, int dtype,
                    float scale, void* out, void* ws, size_t ws_bytes, hipStream_t st);
 
+// orth.hip
+int64_t orthogonalize_ws_bytes(const regcn_matrix* mats, int count);
+int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float b, float c, float eps, void* ws,
+                  size_t ws_bytes, hipStream_t st);
+
 }  // namespace regcn

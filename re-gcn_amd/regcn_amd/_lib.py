@@ -108,6 +108,8 @@ _SIGS = {
     "regcn_embedding": [P, _c_i64, P, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_f, P, P],
     "regcn_embedding_grad_workspace_bytes": [_c_i64, _c_i64, _c_int],
     "regcn_embedding_grad": [P, P, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_f, P, P, _c_sz, P],
+    "regcn_orthogonalize_workspace_bytes": [P, _c_int],
+    "regcn_orthogonalize": [P, _c_int, _c_int, _c_f, _c_f, _c_f, _c_f, P, _c_sz, P],
 }
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # REGCN_F32, REGCN_BF16, REGCN_F16
@@ -119,7 +121,8 @@ _RESTYPE = {"regcn_last_error_string": ctypes.c_char_p, "regcn_hyp_ce_workspace_
             "regcn_row_src_order_workspace_bytes": _c_sz, "regcn_item_src_order_workspace_bytes": _c_sz,
             "regcn_packed_weight_kp_floats": _c_sz,
             "regcn_packed_weight_floats": _c_sz, "regcn_packed_linear_floats": _c_sz,
-            "regcn_packed_k4_floats": _c_sz, "regcn_embedding_grad_workspace_bytes": _c_i64}
+            "regcn_packed_k4_floats": _c_sz, "regcn_embedding_grad_workspace_bytes": _c_i64,
+            "regcn_orthogonalize_workspace_bytes": _c_i64}
 
 _lib = None
 
@@ -196,6 +199,11 @@ class ScoreJob(ctypes.Structure):
     """regcn_score_job (include/regcn_hip.h)."""
     _fields_ = [("q", P), ("cand", P), ("bias", P), ("scale", P), ("margin", P), ("B", _c_int), ("N", _c_int),
                 ("d", _c_int), ("c", _c_f), ("flags", _c_int), ("out", P)]
+
+
+class Matrix(ctypes.Structure):
+    """regcn_matrix (include/regcn_hip.h)."""
+    _fields_ = [("x", P), ("out", P), ("rows", _c_i64), ("cols", _c_i64), ("dtype", _c_int)]
 
 
 class SnapshotDesc(ctypes.Structure):

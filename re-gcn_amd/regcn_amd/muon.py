@@ -1,0 +1,95 @@
+"""The Muon optimiser on HIP: momentum whose two-dimensional updates are orthogonalised.
+
+`orthogonalize` runs the Newton-Schulz iteration
+
+    X = G / (|G|_F + eps);   A = X X^T,  X = a X + (b A + c A A) X,   `steps` times,
+
+on a matrix's shorter side, for any number of matrices of any shapes in one set of launches
+(regcn_orthogonalize): the products run on the fp16 matrix cores as exactly as fp32 products.  With the
+default coefficients the singular values end near 1 (0.7 to 1.2), the singular vectors stay.
+"""
+import functools
+
+import torch
+
+from . import _lib
+
+COEFFS = (3.4445, -4.7750, 2.0315)
+_LIMIT = 4.0
+
+
+@functools.lru_cache(maxsize=64)
+def _check_coeffs(a, b, c, steps):
+    """The operands are held in halves of fp16: the iteration of a singular value from [0, 1] has to stay
+    small.  A grid of 2049 starts, finer than the polynomial turns."""
+    s = torch.linspace(0, 1, 2049, dtype=torch.float64)
+    for _ in range(steps):
+        s = a * s + b * s ** 3 + c * s ** 5
+        if not bool((s.abs() <= _LIMIT).all()):  # NaN and infinities too
+            raise ValueError("coefficients %r leave [-%g, %g] within %d steps" % ((a, b, c), _LIMIT, _LIMIT, steps))
+
+
+def _plan(g):
+    """(contiguous tensor, whether the result is its transpose) of a matrix: a transposed view is taken as
+    the matrix it views (the iteration commutes with transposition)."""
+    if g.dim() != 2:
+        raise ValueError("a matrix has two dimensions (got %s)" % (tuple(g.shape),))
+    if g.dtype not in _lib.DTYPES:
+        raise TypeError("matrices are float32, bfloat16 or float16 (got %s)" % g.dtype)
+    if not g.is_cuda:
+        raise ValueError("matrices must live on a HIP device (got %s); the HIP path has no CPU fallback" % g.device)
+    g = g.detach()
+    if g.is_contiguous():
+        return g, False
+    t = g.t()
+    return (t, True) if t.is_contiguous() else (g.contiguous(), False)
+
+
+def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7):
+    """Newton-Schulz orthogonalisation of a matrix (m x n), of a stack of them (... x m x n), or of a list
+    or tuple of matrices of any shapes and types on one device; the same structure is returned, each result
+    in its matrix's type.  An all-zero matrix stays zero, a matrix without elements is returned as it is;
+    infinities and NaN make their matrix's result NaN.  No gradient flows through the iteration."""
+    steps = int(steps)
+    if not 1 <= steps <= 1000:
+        raise ValueError("1 to 1000 steps (got %d)" % steps)
+    a, b, c = (float(v) for v in coeffs)
+    _check_coeffs(a, b, c, steps)
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("eps must be a number >= 0 (got %r)" % eps)
+    if isinstance(g, torch.Tensor):
+        if g.dim() == 2:
+            return _run([g], steps, a, b, c, eps)[0]
+        if g.dim() < 2:
+            raise ValueError("a matrix has two dimensions (got %s)" % (tuple(g.shape),))
+        m, n = g.shape[-2:]
+        if g.numel() == 0:
+            return g.detach().clone()
+        out = _run(list(g.detach().reshape(-1, m, n).unbind(0)), steps, a, b, c, eps)
+        return torch.stack(out).reshape(g.shape)
+    if not isinstance(g, (list, tuple)) or not all(isinstance(x, torch.Tensor) for x in g):
+        raise TypeError("orthogonalize takes a tensor or a list of matrices (got %s)" % type(g).__name__)
+    out = _run(g, steps, a, b, c, eps)
+    return out if isinstance(g, list) else tuple(out)
+
+
+def _run(mats, steps, a, b, c, eps):
+    plans = [_plan(g) for g in mats]
+    if not plans:
+        return []
+    device = plans[0][0].device
+    if any(p.device != device for p, _ in plans):
+        raise ValueError("the matrices must live on one device")
+    outs = [torch.empty_like(p) for p, _ in plans]
+    live = [k for k, (p, _) in enumerate(plans) if p.numel()]
+    if live:
+        desc = (_lib.Matrix * len(live))()
+        for d, k in zip(desc, live):
+            p = plans[k][0]
+            d.x, d.out, d.rows, d.cols, d.dtype = p.data_ptr(), outs[k].data_ptr(), p.shape[0], p.shape[1], \
+                _lib.DTYPES[p.dtype]
+        size = _lib.lib().regcn_orthogonalize_workspace_bytes(desc, len(live))
+        ws = torch.empty(size, device=device, dtype=torch.uint8)
+        _lib.launch("regcn_orthogonalize", device, desc, len(live), steps, a, b, c, eps, ws.data_ptr(), size)
+    return [o.t() if t else o for o, (_, t) in zip(outs, plans)]
