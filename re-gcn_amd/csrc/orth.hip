@@ -29,7 +29,7 @@ namespace {
 constexpr int MAXM = 32;      // matrices in a set of launches
 constexpr int THR = 256;      // four waves, 2 x 2 over the tile
 constexpr int KSTEP = 32;     // k of a stage: a 128-byte line of each row
-constexpr int NORM_WGS = 64;  // most partial sums of a norm
+constexpr int NORM_WGS = 1024;  // most partial sums of a norm
 constexpr float LO = 2048.f;  // scale of the low halves
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -76,8 +76,9 @@ struct Parts {
 
 // This workgroup's matrix; wg becomes its index within it.
 __device__ __forceinline__ int find_mat(const Job& j, int& wg) {
-  int q = 0;
-  while (q + 1 < j.count && wg >= j.start[q + 1]) ++q;
+  // one load a lane and a ballot: a loop over the starts would wait for each in turn
+  const int lane = threadIdx.x & 63;
+  const int q = __popcll(__ballot(lane < j.count && wg >= j.start[lane + 1]));
   wg -= j.start[q];
   return q;
 }
@@ -154,7 +155,10 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
   const int lane = threadIdx.x & 63;
   // every wave sums the partial norms in the same order
   const double* part = (const double*)(q.ws + w.norm);
-  double s = lane < norm_parts((int64_t)q.m * q.n) ? part[lane] : 0.0;
+  const int parts = norm_parts((int64_t)q.m * q.n);
+  double s = 0;
+#pragma unroll 16
+  for (int p = lane; p < parts; p += WAVE) s += part[p];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   const float den = (float)sqrt(s) + job.eps;
@@ -272,7 +276,7 @@ template <int T>
 __device__ __forceinline__ void finish(float* c, const char* old, float alpha, float beta, char* dst, char* dst_t,
                                        int64_t ld, int64_t ld_t) {
   constexpr int G = T / 8;
-  for (int it = threadIdx.x; it < T * G; it += THR) {
+  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
 #pragma unroll
@@ -289,7 +293,7 @@ __device__ __forceinline__ void finish(float* c, const char* old, float alpha, f
   }
   if (!dst_t) return;
   __syncthreads();
-  for (int it = threadIdx.x; it < T * G; it += THR) {
+  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
     const int col = it / 64 * 16 % T + (it & 15), g = it / 64 * 16 / T * 4 + (it >> 4 & 3);
     float v[8];
 #pragma unroll
@@ -321,7 +325,7 @@ __device__ __forceinline__ void store_out(const Mat& q, int64_t at, const float 
 template <int T>
 __device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* old, float alpha, int64_t ld, int i0, int j0) {
   constexpr int G = T / 8;
-  for (int it = threadIdx.x; it < T * G; it += THR) {
+  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
     load_group(x, old + r * ld + g * 32);
@@ -334,7 +338,7 @@ __device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* o
   }
   if (!q.trans) return;
   __syncthreads();
-  for (int it = threadIdx.x; it < T * G; it += THR) {
+  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
     const int col = it / 64 * 16 % T + (it & 15), g = it / 64 * 16 / T * 4 + (it >> 4 & 3);
     float v[8];
 #pragma unroll
@@ -376,21 +380,23 @@ __global__ __launch_bounds__(THR, 2) void k_gram(Job job) {
   finish<T>(c, nullptr, 0.f, 1.f, A + i * T * la + j * T * 4, i == j ? nullptr : A + j * T * la + i * T * 4, la, la);
 }
 
-// The pieces of k of a tile added up in order.
+// The pieces of k of a tile added up in order: a thread per 4 columns, its pieces' loads under way together.
 template <int T>
-__global__ __launch_bounds__(THR) void k_gram_sum(Job job) {
+__global__ __launch_bounds__(T * T / 4 < 1024 ? T * T / 4 : 1024) void k_gram_sum(Job job) {
   __shared__ __align__(16) float c[T * (T + 1)];
   int wg = blockIdx.x, i, j;
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<T> w(q);
   const int nt = w.mp / T, tri = nt * (nt + 1) / 2;
   triangle(wg, nt, i, j);
-  const float* part = (const float*)(q.ws + w.split) + (int64_t)wg * T * T;
-  for (int it = threadIdx.x; it < T * T; it += THR) {
-    float v = part[it];
+  const f4* part = (const f4*)(q.ws + w.split) + (int64_t)wg * (T * T / 4);
+  for (int it = threadIdx.x; it < T * T / 4; it += blockDim.x) {
+    f4 v = part[it];
 #pragma unroll 8
-    for (int s = 1; s < q.splits; ++s) v += part[(int64_t)s * tri * T * T + it];
-    c[it / T * (T + 1) + it % T] = v;
+    for (int s = 1; s < q.splits; ++s) v += part[(int64_t)s * tri * (T * T / 4) + it];
+    const int at = it * 4 / T * (T + 1) + it * 4 % T;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[at + e] = v[e];
   }
   __syncthreads();
   const int64_t la = (int64_t)w.mp * 4;
@@ -438,10 +444,11 @@ bool wide_tiles(const Mat& q) { return (int64_t)((q.m + 127) / 128) * ((q.n + 12
 
 int tile_of(const Mat& q) { return wide_tiles(q) ? 128 : 64; }
 
-// Pieces of k in X X^T: enough for about 512 workgroups, each of at least 8 k-steps.
+// Pieces of k in X X^T: enough for about 512 workgroups, each of at least 24 k-steps (about 6 us: the
+// second launch that adds them up costs 4).
 int gram_splits(const Mat& q) {
   const int t = tile_of(q), nt = (q.m + t - 1) / t, tri = nt * (nt + 1) / 2, steps = pad_to(q.n, t) / KSTEP;
-  return std::max(1, std::min({512 / tri, steps / 8, 32}));
+  return std::max(1, std::min({512 / tri, steps / 24, 32}));
 }
 
 template <typename F>
@@ -462,7 +469,7 @@ int run_set(Job& job, int steps, hipStream_t st) {
     n = layout(job, [&](const Mat& q) { return tri(q) * q.splits; });
     k_gram<T><<<n, THR, 0, st>>>(job);
     n = layout(job, [&](const Mat& q) { return q.splits > 1 ? tri(q) : 0; });
-    if (n) k_gram_sum<T><<<n, THR, 0, st>>>(job);
+    if (n) k_gram_sum<T><<<n, std::min(1024, T * T / 4), 0, st>>>(job);
     n = layout(job, tri);
     k_poly<T><<<n, THR, 0, st>>>(job);
     n = layout(job, [](const Mat& q) { return pad_to(q.m, T) / T * (pad_to(q.n, T) / T); });
