@@ -871,6 +871,32 @@ int64_t regcn_orthogonalize_workspace_bytes(const regcn_matrix* mats, int32_t n_
 int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps, float a, float b, float c, float eps,
                         void* workspace, size_t ws_bytes, void* stream);
 
+/* ---- Sampling ids from scores -------------------------------------------------------------- */
+typedef struct regcn_sample_desc {
+  const void* score;              /* rows x cols of `dtype`, rows `ld` elements apart */
+  int64_t ld;
+  int32_t rows, cols, draws, dtype; /* cols up to 2^24 */
+  const void* u;                  /* rows x draws numbers in [0, 1): float, or double (u_wide) */
+  int32_t u_wide;
+  int32_t top_k;                  /* <= 0 or >= cols: off */
+  double temperature;             /* not above 0: the first of the order */
+  double top_p, min_p;            /* >= 1: off; <= 0: off */
+  const float* temperature_rows;  /* one per row in place of the number above, or NULL */
+  const int32_t* top_k_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  int64_t* ids;                   /* rows x draws: the drawn column, -1 for a row without a score to take */
+  float* logp;                    /* rows x draws: log of the draw's probability (-inf with -1), or NULL */
+  void* workspace;                /* regcn_sample_workspace_bytes (0: may be NULL) */
+  size_t ws_bytes;
+} regcn_sample_desc;
+/* Per row: weights exp((s - max) / temperature); kept are, in the order "larger score first, ties by lower
+ * column", the first top_k, of those the shortest prefix whose weights reach top_p of their sum, and of those
+ * the weights >= min_p (the first is always kept); a draw is the lowest column whose running sum (by column)
+ * of kept weights exceeds u times their sum.  NaN and -inf scores are never taken; +inf shares all weight. */
+int64_t regcn_sample_workspace_bytes(int32_t rows, int32_t cols, int32_t dtype);
+int regcn_sample(const regcn_sample_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -801,4 +801,10 @@ int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps,
   return orthogonalize(mats, n_mats, steps, a, b, c, eps, workspace, ws_bytes, ST(s));
 }
 
+int64_t regcn_sample_workspace_bytes(int32_t rows, int32_t cols, int32_t dtype) { return sample_ws_bytes(rows, cols, dtype); }
+int regcn_sample(const regcn_sample_desc* desc, void* s) {
+  if (!desc) return set_error(REGCN_EINVAL, "null desc");
+  return sample(*desc, ST(s));
+}
+
 }  // extern "C"

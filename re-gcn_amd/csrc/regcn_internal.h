@@ -365,4 +365,8 @@ int64_t orthogonalize_ws_bytes(const regcn_matrix* mats, int count);
 int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float b, float c, float eps, void* ws,
                   size_t ws_bytes, hipStream_t st);
 
+// sample.hip
+int64_t sample_ws_bytes(int rows, int cols, int dtype);
+int sample(const regcn_sample_desc& d, hipStream_t st);
+
 }  // namespace regcn

@@ -110,6 +110,8 @@ _SIGS = {
     "regcn_embedding_grad": [P, P, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_f, P, P, _c_sz, P],
     "regcn_orthogonalize_workspace_bytes": [P, _c_int],
     "regcn_orthogonalize": [P, _c_int, _c_int, _c_f, _c_f, _c_f, _c_f, P, _c_sz, P],
+    "regcn_sample_workspace_bytes": [_c_int, _c_int, _c_int],
+    "regcn_sample": [P, P],
 }
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # REGCN_F32, REGCN_BF16, REGCN_F16
@@ -122,7 +124,7 @@ _RESTYPE = {"regcn_last_error_string": ctypes.c_char_p, "regcn_hyp_ce_workspace_
             "regcn_packed_weight_kp_floats": _c_sz,
             "regcn_packed_weight_floats": _c_sz, "regcn_packed_linear_floats": _c_sz,
             "regcn_packed_k4_floats": _c_sz, "regcn_embedding_grad_workspace_bytes": _c_i64,
-            "regcn_orthogonalize_workspace_bytes": _c_i64}
+            "regcn_orthogonalize_workspace_bytes": _c_i64, "regcn_sample_workspace_bytes": _c_i64}
 
 _lib = None
 
@@ -204,6 +206,14 @@ class ScoreJob(ctypes.Structure):
 class Matrix(ctypes.Structure):
     """regcn_matrix (include/regcn_hip.h)."""
     _fields_ = [("x", P), ("out", P), ("rows", _c_i64), ("cols", _c_i64), ("dtype", _c_int)]
+
+
+class SampleDesc(ctypes.Structure):
+    """regcn_sample_desc (include/regcn_hip.h)."""
+    _fields_ = [("score", P), ("ld", _c_i64), ("rows", _c_int), ("cols", _c_int), ("draws", _c_int), ("dtype", _c_int),
+                ("u", P), ("u_wide", _c_int), ("top_k", _c_int), ("temperature", ctypes.c_double),
+                ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("temperature_rows", P), ("top_k_rows", P),
+                ("top_p_rows", P), ("min_p_rows", P), ("ids", P), ("logp", P), ("workspace", P), ("ws_bytes", _c_sz)]
 
 
 class SnapshotDesc(ctypes.Structure):

@@ -13,6 +13,8 @@ rank).  As in the reference (filter_score / filter_score_r write into a view of 
 rgcn/utils.py:51-75), `score` leaves get_total_rank with the other true answers set to
 -1e7, so `construct_snap` under --multi-step picks its top-k from the filtered scores.
 """
+import ctypes
+
 import numpy as np
 import torch
 
@@ -83,6 +85,85 @@ def get_total_rank(test_triples, score, all_ans, eval_bz, rel_predict=0):
     mrr = torch.mean(1.0 / rank.float())
     filter_mrr = torch.mean(1.0 / filter_rank.float())
     return filter_mrr.item(), mrr.item(), rank, filter_rank
+
+
+_SAMPLE_MAX_COLS = 1 << 24
+
+
+def _limit(value, name, rows, device, dtype, low, high, high_in=True):
+    """(number, device tensor of one per row or None) of a sampling limit."""
+    if isinstance(value, torch.Tensor) and value.dim() > 0:
+        if value.shape != (rows,) or value.device != device:
+            raise ValueError("%s must be one number or a tensor of %d on %s (got %s on %s)"
+                             % (name, rows, device, tuple(value.shape), value.device))
+        return 0, value.to(dtype).contiguous()
+    v = float(value)
+    if not (low <= v < high or high_in and v == high):
+        raise ValueError("%s must lie between %g and %g (got %r)" % (name, low, high, value))
+    return v, None
+
+
+def sample(score, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp=False):
+    """Ids drawn from scores (B x N, or N for one row; fp32, bf16 or fp16) at the numbers u in [0, 1)
+    (B, or B x S for S draws a row; fp32 or fp64), one HIP launch a call (regcn_sample).  Per row, with
+    weights w = exp((score - max) / temperature): in the order "larger score first, ties by lower id" are
+    kept the first `top_k` (0: all), of those the shortest prefix holding `top_p` of their weight, and of
+    those w >= `min_p` (the first is always kept); a draw is the lowest id whose running sum, by id, of kept
+    weights exceeds u times their sum.  Sums are exact, so equal inputs give equal ids on every call.
+
+    NaN and -inf scores are never drawn and a row of them gives -1; temperature 0 takes the best id.
+    temperature, top_k, top_p and min_p may each be a tensor of one value per row (not checked: a
+    temperature that is not above 0 takes the best id, top_k <= 0, top_p >= 1 and min_p <= 0 are off).
+    Returns int64 ids in u's shape, with return_logp also the log of each draw's probability among the
+    kept (fp32, -inf where the id is -1)."""
+    if not isinstance(score, torch.Tensor) or not isinstance(u, torch.Tensor):
+        raise TypeError("sample takes tensors (score: %s, u: %s)" % (type(score).__name__, type(u).__name__))
+    if score.dim() not in (1, 2) or u.dim() > score.dim():
+        raise ValueError("score is B x N with u of B or B x S, or N with u of S or one number (got %s, %s)"
+                         % (tuple(score.shape), tuple(u.shape)))
+    if score.dtype not in _lib.DTYPES:
+        raise TypeError("score must be float32, bfloat16 or float16 (got %s)" % score.dtype)
+    if u.dtype not in (torch.float32, torch.float64):
+        raise TypeError("u must be float32 or float64 (got %s)" % u.dtype)
+    rows = score.shape[0] if score.dim() == 2 else 1
+    if score.dim() == 2 and (u.dim() == 0 or u.shape[0] != rows):
+        raise ValueError("u has %s, score %d rows" % (tuple(u.shape), rows))
+    cols = score.shape[-1]
+    if cols > _SAMPLE_MAX_COLS:
+        raise ValueError("rows of up to %d scores (got %d)" % (_SAMPLE_MAX_COLS, cols))
+    dev = score.device
+    t, t_rows = _limit(temperature, "temperature", rows, dev, torch.float32, 0.0, float("inf"), False)
+    k, k_rows = _limit(top_k, "top_k", rows, dev, torch.int32, 0, 2 ** 31 - 1)
+    p, p_rows = _limit(top_p, "top_p", rows, dev, torch.float32, 0.0, 1.0)
+    m, m_rows = _limit(min_p, "min_p", rows, dev, torch.float32, 0.0, 1.0)
+    if not score.is_cuda or u.device != dev:
+        raise ValueError("score and u must live on one HIP device (got %s, %s); the HIP path has no CPU fallback"
+                         % (dev, u.device))
+    score, u = score.detach(), u.detach().contiguous()
+    if cols > 1 and score.stride(-1) != 1 or rows > 1 and score.stride(0) < cols:
+        score = score.contiguous()
+    ids = torch.empty(u.shape, device=dev, dtype=torch.int64)
+    logp = torch.empty(u.shape, device=dev, dtype=torch.float32) if return_logp else None
+    draws = u.numel() // rows if rows else 0
+    if cols == 0:
+        ids.fill_(-1)
+        if return_logp:
+            logp.fill_(-float("inf"))
+    elif draws:
+        d = _lib.SampleDesc()
+        d.score, d.ld, d.rows, d.cols, d.draws = score.data_ptr(), score.stride(0) if rows > 1 else cols, rows, cols, draws
+        d.dtype, d.u, d.u_wide, d.top_k = _lib.DTYPES[score.dtype], u.data_ptr(), u.dtype == torch.float64, int(k)
+        d.temperature, d.top_p, d.min_p, d.ids = t, p, m, ids.data_ptr()
+        for name, v in (("temperature_rows", t_rows), ("top_k_rows", k_rows), ("top_p_rows", p_rows),
+                        ("min_p_rows", m_rows), ("logp", logp)):
+            if v is not None:
+                setattr(d, name, v.data_ptr())
+        d.ws_bytes = _lib.lib().regcn_sample_workspace_bytes(rows, cols, d.dtype)
+        if d.ws_bytes:
+            ws = torch.empty(d.ws_bytes, device=dev, dtype=torch.uint8)
+            d.workspace = ws.data_ptr()
+        _lib.launch("regcn_sample", dev, ctypes.byref(d))
+    return (ids, logp) if return_logp else ids
 
 
 def stat_ranks(rank_list, method):

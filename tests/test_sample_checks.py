@@ -1,0 +1,44 @@
+"""Refusals of ranking.sample and its C entry (no GPU: every call raises before it reaches one)."""
+import ctypes
+
+import pytest
+import torch
+
+from regcn_amd import _lib, ranking
+
+S, U = torch.zeros(3, 10), torch.zeros(3)
+
+
+@pytest.mark.parametrize("args,kw,err", [
+    ((S, U), {}, ValueError), ((S.numpy(), U), {}, TypeError), ((S, 0.5), {}, TypeError), ((S.double(), U), {}, TypeError),
+    ((S, U.half()), {}, TypeError), ((S[None], U), {}, ValueError), ((S, U[:2]), {}, ValueError), ((S[0], S), {}, ValueError),
+    ((S, torch.tensor(0.5)), {}, ValueError), ((S, U), dict(temperature=-1.0), ValueError),
+    ((S, U), dict(temperature=float("nan")), ValueError), ((S, U), dict(temperature=float("inf")), ValueError),
+    ((S, U), dict(top_k=-1), ValueError), ((S, U), dict(top_p=1.5), ValueError), ((S, U), dict(top_p=-0.1), ValueError),
+    ((S, U), dict(min_p=2.0), ValueError), ((S, U), dict(min_p=float("nan")), ValueError),
+    ((S, U), dict(top_p=torch.ones(2)), ValueError),
+    ((torch.zeros(1, 1).expand(1, (1 << 24) + 1), U[:1]), {}, ValueError)])
+def test_sample_refuses(args, kw, err):
+    with pytest.raises(err):
+        ranking.sample(*args, **kw)
+
+
+def test_c_entry_refuses():
+    lib = _lib.lib()
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(buf)
+
+    def call(**kw):
+        d = _lib.SampleDesc()
+        d.score, d.u, d.ids, d.ld, d.rows, d.cols, d.draws, d.temperature, d.top_p = p, p, p, 10, 3, 10, 1, 1.0, 1.0
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return lib.regcn_sample(ctypes.byref(d), None)
+
+    for kw in (dict(score=None), dict(u=None), dict(ids=None), dict(rows=-1), dict(cols=-2), dict(draws=-1), dict(dtype=3),
+               dict(dtype=-1), dict(ld=9), dict(cols=(1 << 24) + 1, ld=1 << 25)):
+        assert call(**kw) < 0, kw
+    assert b"sample" in lib.regcn_last_error_string()
+    assert call(rows=0) == 0 and call(draws=0) == 0
+    assert lib.regcn_sample(None, None) < 0
+    assert lib.regcn_sample_workspace_bytes(0, 0, 0) >= 0
