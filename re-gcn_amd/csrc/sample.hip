@@ -7,17 +7,20 @@
 //   id(u) = the lowest i whose running sum (by index) of kept weights exceeds u * (sum of kept weights)
 // T <= 0 takes the first of the order.  A row without a score to take gives -1.
 //
-// Weights are whole numbers: round(w 2^S) with 2^S N <= 2^63 (S <= 52), from a 64-bit exp.  Their sums are
+// Weights are whole numbers: round(w 2^S) with 2^S N <= 2^63 (S <= 51), from a 64-bit exp.  Their sums are
 // exact in any order, so histograms by atomics, partial sums and prefix sums agree bit for bit.
 //
 // No sort.  Scores become 32-bit keys of the same order.  Each of k and p asks for the place in the order
 // where a running sum (of ones, of weights) reaches a target: a radix descent over the keys finds the
 // key (histograms of 11 bits; a round after the first touches the elements of one bin only), and where several
-// elements share that key, how many of them, lowest indices first.  So a kept set is {key > K} and
-// {key = K, index <= I}.
+// elements share that key, a descent over their indices finds the last one kept.  So a kept set is
+// {key > K} and {key = K, index <= I}.
 //
-// A workgroup takes a row.  Up to 32768 scores stay in its registers as keys (one read of the scores);
-// longer rows are read again in each pass, from the caches where they fit.
+// k_sample: a workgroup takes a row.  Up to 32768 scores stay in its LDS as keys (one read of the scores;
+// in registers, the compiler spilled them around the 64-bit exponentials); longer rows are read again in each
+// pass.
+// Few long rows: several workgroups take a row's segments, in launches that pass histograms, the members of
+// the bin in question and segment sums through a workspace (k_spread_*).
 #include "elem.h"
 #include "regcn_internal.h"
 
@@ -25,7 +28,7 @@ namespace regcn {
 namespace {
 
 constexpr int HBITS = 11, HBINS = 1 << HBITS;
-constexpr int MAX_KEYS = 32;  // keys a thread holds
+constexpr int ROW_KEYS = 32768;  // scores of a row held in LDS
 constexpr uint32_t ALL = 0xffffffffu;
 constexpr int CHUNKS = 4096;  // running sums of kept weights kept in LDS, at most
 constexpr int MAX_COLS = 1 << 24;
@@ -44,9 +47,13 @@ struct RowArgs {
 };
 
 struct Limits {
-  double inv_t, top_p, min_p;
-  uint32_t top_k;  // ALL: off
+  double inv_t, top_p, min_w;  // min_w: min_p 2^S
+  uint32_t top_k;              // ALL: off
   int shift;
+  // set once the row's largest score is known
+  uint32_t kmax;
+  double top;
+  bool ties_only;  // an infinite score, or a temperature whose inverse is: weight only on the largest
 };
 
 __device__ __forceinline__ Limits row_limits(const RowArgs& a, int row) {
@@ -54,7 +61,7 @@ __device__ __forceinline__ Limits row_limits(const RowArgs& a, int row) {
   const double t = a.temperature_v ? (double)a.temperature_v[row] : a.temperature;
   const int k = a.top_k_v ? a.top_k_v[row] : a.top_k;
   l.top_p = a.top_p_v ? (double)a.top_p_v[row] : a.top_p;
-  l.min_p = a.min_p_v ? (double)a.min_p_v[row] : a.min_p;
+  l.min_w = __builtin_ldexp(a.min_p_v ? (double)a.min_p_v[row] : a.min_p, a.shift);
   l.top_k = k > 0 && k < a.cols ? (uint32_t)k : ALL;
   l.inv_t = 1.0 / t;
   if (!(t > 0)) {  // greedy
@@ -73,17 +80,20 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 }
 __device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : ALL)); }
 
-// round(exp(x) 2^S) for x = (s - top) / T <= 0, and exp(x) itself.  exp(x) = 2^n p(r), r = x - n ln 2 in
-// two parts, |r| <= ln 2 / 2; p is the Taylor polynomial of degree 13 (remainder below 2^-57).
-__device__ __forceinline__ uint64_t weight(uint32_t key, float top, const Limits& l, double* value = nullptr) {
-  const float s = key_score(key);
-  double x = s == top ? 0.0 : ((double)s - (double)top) * l.inv_t;
-  x = x > -700.0 ? x : -700.0;
+__device__ __forceinline__ void set_top(Limits& l, uint32_t kmax) {
+  l.kmax = kmax;
+  l.top = (double)key_score(kmax);
+  l.ties_only = !(fabs(l.top) < __builtin_inf() && l.inv_t < __builtin_inf());
+}
+
+// exp(x) 2^S for x = (s - top) / T <= 0.  exp(x) = 2^n p(r), r = x - n ln 2 in two parts, |r| <= ln 2 / 2;
+// p is the Taylor polynomial of degree 12 (remainder below 2^-52 of p).
+__device__ __forceinline__ double scaled_exp(uint32_t key, const Limits& l) {
+  const double x = fmax(((double)key_score(key) - l.top) * l.inv_t, -700.0);
   const double n = __builtin_rint(x * 1.4426950408889634074);
   double r = fma(n, -6.93147180369123816490e-01, x);
   r = fma(n, -1.90821492927058770002e-10, r);
-  double p = 1.0 / 6227020800.0;
-  p = fma(p, r, 1.0 / 479001600.0);
+  double p = 1.0 / 479001600.0;
   p = fma(p, r, 1.0 / 39916800.0);
   p = fma(p, r, 1.0 / 3628800.0);
   p = fma(p, r, 1.0 / 362880.0);
@@ -96,14 +106,15 @@ __device__ __forceinline__ uint64_t weight(uint32_t key, float top, const Limits
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
-  const int e = (int)n;
-  if (value) *value = __builtin_ldexp(p, e);
-  // p's 53-bit number, shifted so that its last bit is 2^-S, to nearest
-  const uint64_t bits = __double_as_longlong(p);
-  const uint64_t m = (bits & ((1ull << 52) - 1)) | (1ull << 52);
-  const int sh = 52 - ((int)(bits >> 52) - 1023) - e - l.shift;  // >= -1 (p in [0.7, 1.42), e <= 0)
-  if (sh <= 0) return m << -sh;
-  return sh > 54 ? 0 : (m + (1ull << (sh - 1))) >> sh;
+  return __builtin_ldexp(p, (int)n + l.shift);
+}
+
+// To the nearest whole number: adding 2^52 to a number up to 2^51 leaves it in the low bits.
+__device__ __forceinline__ uint64_t whole(double v) { return __double_as_longlong(v + 0x1p52) & ((1ull << 52) - 1); }
+
+__device__ __forceinline__ uint64_t weight(uint32_t key, const Limits& l) {
+  if (l.ties_only) return key == l.kmax ? 1ull << l.shift : 0;
+  return whole(scaled_exp(key, l));
 }
 
 // A place in the order: everything with a larger key, and of its own key the indices up to idx.
@@ -113,14 +124,21 @@ struct Cut {
   __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= idx); }
 };
 
+// The weight of an element, 0 where a limit leaves it out.
+__device__ __forceinline__ uint64_t kept_weight(uint32_t key, int idx, const Cut& cut, const Limits& l) {
+  if (!key || !cut.keeps(key, idx)) return 0;
+  if (l.ties_only) return key == l.kmax ? 1ull << l.shift : 0;
+  const double v = scaled_exp(key, l);
+  return v >= l.min_w || key == l.kmax ? whole(v) : 0;
+}
+
 template <int THR>
 struct Shared {
   uint64_t hist[HBINS];
   uint64_t wave[THR / WAVE];
   uint32_t kmax[THR / WAVE], kmin[THR / WAVE];
-  uint64_t above, tie;
+  uint64_t above, sum;
   uint32_t bin;
-  int idx;
 };
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
@@ -160,198 +178,256 @@ __device__ __forceinline__ uint64_t block_scan64(uint64_t v, uint64_t* wave, uin
   return base + inc - v;
 }
 
-// The row as this workgroup sees it: piece q of thread t holds the VE scores from (q THR + t) VE on.
-template <typename T, int THR, int NP>  // NP: pieces in registers, 0: read again each time
+// The row as this workgroup sees it: piece q of thread t holds the VE scores from (q THR + t) VE on.  With
+// KEYS > 0 it is read once, into `keys` (LDS); otherwise again in each pass.
+template <typename T, int THR, int KEYS>
 struct Row {
-  static constexpr int VE = Piece<T>::VE;
+  static constexpr int VE = KEYS > 0 ? 4 : Piece<T>::VE;
   const T* p;
+  uint32_t* keys;
   int n, pieces;  // pieces a thread
-  uint32_t keys[NP > 0 ? NP : 1][VE];
 
-  __device__ __forceinline__ void read(int q, uint32_t (&k)[VE]) const {
-    const int i0 = (q * THR + threadIdx.x) * VE;
-    float x[VE];
+  template <int N>
+  __device__ __forceinline__ void load(int i0, uint32_t (&k)[N]) const {
+    static_assert(N == Piece<T>::VE, "a piece of the type");
+    float x[N];
     const int m = n - i0;
     if (m > 0) load_piece<T>(x, p + i0, m);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) k[e] = e < m ? score_key(x[e]) : 0u;
+    for (int e = 0; e < N; ++e) k[e] = e < m ? score_key(x[e]) : 0u;
   }
-  __device__ __forceinline__ void init(const T* row, int cols) {
+  // the keys from i0 (a multiple of VE) on; 0 past the row's end
+  __device__ __forceinline__ void read_at(int i0, uint32_t (&k)[VE]) const {
+    if constexpr (KEYS > 0) {
+      const uint4 v = i0 < KEYS ? *reinterpret_cast<const uint4*>(keys + i0) : make_uint4(0, 0, 0, 0);
+      k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+    } else {
+      load(i0, k);
+    }
+  }
+  __device__ __forceinline__ void init(const T* row, int cols, uint32_t* lds) {
     p = row;
     n = cols;
+    keys = lds;
     pieces = (cols + THR * VE - 1) / (THR * VE);
-    if (NP > 0) {
+    if constexpr (KEYS > 0) {
+      constexpr int PV = Piece<T>::VE;
+#pragma unroll 8
+      for (int i0 = (int)threadIdx.x * PV; i0 < pieces * THR * VE; i0 += THR * PV) {
+        uint32_t k[PV];
+        load(i0, k);
 #pragma unroll
-      for (int q = 0; q < NP; ++q) read(q, keys[q]);
+        for (int e = 0; e < PV; e += 4)
+          *reinterpret_cast<uint4*>(keys + i0 + e) = make_uint4(k[e], k[e + 1], k[e + 2], k[e + 3]);
+      }
+      __syncthreads();
     }
   }
   // f(q, first index, keys of the piece) for every piece
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    if (NP > 0) {
-#pragma unroll
-      for (int q = 0; q < NP; ++q) f(q, (q * THR + (int)threadIdx.x) * VE, keys[q]);
-    } else {
-      for (int q = 0; q < pieces; ++q) {
-        uint32_t k[VE];
-        read(q, k);
-        f(q, (q * THR + (int)threadIdx.x) * VE, k);
-      }
+  __device__ __forceinline__ void pieces_of(F f) const {
+    for (int q = 0; q < pieces; ++q) {
+      uint32_t k[VE];
+      const int i0 = (q * THR + (int)threadIdx.x) * VE;
+      read_at(i0, k);
+      f(q, i0, k);
     }
+  }
+  // f(key, index) for every element
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    pieces_of([&](int, int i0, const uint32_t* k) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (k[e]) f(k[e], i0 + e);
+    });
   }
 };
 
-// The cut where the running sum of `value` over the order first reaches the target, among the elements that
-// `in` admits: an element is kept when the sum before it is below the target.  target_of(total) gives the
-// target once the total is known (after the first histogram).
-template <typename R, int THR, typename In, typename Value, typename Target>
-__device__ Cut find_cut(const R& row, Shared<THR>& sh, uint32_t kmin, uint32_t kmax, In in, Value value, Target target_of) {
-  constexpr int PER = HBINS / THR;
-  uint32_t lo = kmin, hi = kmax;  // the keys still in question
-  uint64_t above = 0, target = 0;
-  bool first = true;
-  for (;;) {
+// Elements in a list, in no order.
+template <int THR>
+struct List {
+  const uint2* p;
+  int n;
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x; i < n; i += THR) f(p[i].x, (int)p[i].y);
+  }
+};
+
+// The bin of sh.hist in which the running sum, `above` before bin 0, reaches the target: into sh.bin, with the
+// sum before it in sh.above and its own in sh.sum (1 <= target - above <= the histogram's total).  target_of
+// gives the target from the total.
+template <int THR, int BINS, typename Target>
+__device__ __forceinline__ uint64_t find_bin(Shared<THR>& sh, const uint64_t* hist, uint64_t above, Target target_of) {
+  constexpr int PER = BINS / THR;
+  uint64_t own = 0, total, h[PER];
+#pragma unroll
+  for (int b = 0; b < PER; ++b) own += h[b] = hist[threadIdx.x * PER + b];
+  uint64_t before = above + block_scan64<THR>(own, sh.wave, &total);
+  const uint64_t target = target_of(total);
+#pragma unroll
+  for (int b = 0; b < PER; ++b) {
+    if (before < target && before + h[b] >= target) {  // one thread's
+      sh.above = before;
+      sh.bin = threadIdx.x * PER + b;
+      sh.sum = h[b];
+    }
+    before += h[b];
+  }
+  __syncthreads();
+  return target;
+}
+
+struct Place {
+  uint32_t key;
+  uint64_t above, sum, target;  // sums before the key, of the key
+};
+
+// Radix descent in decreasing order of mapped keys in [lo, hi]: the key at which the running sum of values,
+// starting from `above`, reaches the target.  each(f) calls f(mapped key, value functor) for the elements.
+template <int THR, typename Each, typename Target>
+__device__ Place descend(Shared<THR>& sh, uint32_t lo, uint32_t hi, uint64_t above, Each each, Target target_of) {
+  uint64_t target = 0;
+  for (bool first = true;; first = false) {
     const uint32_t range = hi - lo;
     const int bits = range ? 32 - __builtin_clz(range) : 0;
     const int shift = bits > HBITS ? bits - HBITS : 0;
     for (int b = threadIdx.x; b < HBINS; b += THR) sh.hist[b] = 0;
     __syncthreads();
-    row.each([&](int, int i0, const uint32_t* k) {
-#pragma unroll
-      for (int e = 0; e < R::VE; ++e)
-        if (k[e] >= lo && k[e] <= hi && k[e] && in(k[e], i0 + e))
-          atomicAdd((unsigned long long*)&sh.hist[(hi - k[e]) >> shift], (unsigned long long)value(k[e]));
+    each([&](uint32_t k, auto value) {
+      if (k >= lo && k <= hi)
+        atomicAdd((unsigned long long*)&sh.hist[(hi - k) >> shift], (unsigned long long)value());
     });
     __syncthreads();
-    uint64_t own = 0, total;
-    uint64_t h[PER];
-#pragma unroll
-    for (int b = 0; b < PER; ++b) own += h[b] = sh.hist[threadIdx.x * PER + b];
-    uint64_t before = above + block_scan64<THR>(own, sh.wave, &total);
-    if (first) target = target_of(total);
-    first = false;
-    // the bin in which the sum reaches the target: exactly one thread finds it (the target is at most the total)
-#pragma unroll
-    for (int b = 0; b < PER; ++b) {
-      if (before < target && before + h[b] >= target) {
-        sh.above = before;
-        sh.bin = threadIdx.x * PER + b;
-        sh.tie = h[b];
-      }
-      before += h[b];
-    }
-    __syncthreads();
+    const uint64_t t = find_bin<THR, HBINS>(sh, sh.hist, above, [&](uint64_t total) { return first ? target_of(total) : target; });
+    target = t;
     above = sh.above;
-    const uint32_t top = hi - (sh.bin << shift);
-    const uint32_t low = (1u << shift) - 1;
+    const uint32_t top = hi - (sh.bin << shift), low = (1u << shift) - 1;
     lo = max(lo, top >= low ? top - low : 0);
     hi = top;
     if (shift == 0) break;
   }
-  // one key left: its elements each add the same; the lowest indices are kept
-  const uint64_t one = value(hi), need = one ? (target - above + one - 1) / one : 1, have = one ? sh.tie / one : 1;
-  Cut cut{hi, 0x7fffffff};
-  if (need < have) {
-    uint64_t seen = 0;
-    if (threadIdx.x == 0) sh.idx = 0x7fffffff;
-    for (int q = 0; q < row.pieces; ++q) {  // THR * VE elements at a time, in index order
-      int mine = 0;
-      uint32_t k[R::VE];
-      const int i0 = (q * THR + (int)threadIdx.x) * R::VE;
-      row.read(q, k);
-#pragma unroll
-      for (int e = 0; e < R::VE; ++e) mine += k[e] == hi && in(k[e], i0 + e);
-      uint64_t total;
-      uint64_t at = seen + block_scan64<THR>((uint64_t)mine, sh.wave, &total);
-#pragma unroll
-      for (int e = 0; e < R::VE; ++e)
-        if (k[e] == hi && in(k[e], i0 + e) && ++at == need) sh.idx = i0 + e;
-      seen += total;
-      if (seen >= need) break;
-    }
-    __syncthreads();
-    cut.idx = sh.idx;
-  }
-  __syncthreads();  // hist and the rest may be written again
-  return cut;
+  const Place p{hi, above, sh.sum, target};
+  __syncthreads();  // sh may be written again
+  return p;
 }
 
-template <typename T, int THR, int NP>
-__global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
-  constexpr int VE = Piece<T>::VE, WAVES = THR / WAVE;
-  const int subs = (a.cols + WAVE * VE - 1) / (WAVE * VE);  // a wave's pieces: WAVE * VE consecutive scores
-  const int group = (subs + CHUNKS - 1) / CHUNKS, chunks = (subs + group - 1) / group;
-  __shared__ Shared<THR> sh;
-  extern __shared__ uint64_t chunk[];  // running kept weight after each chunk of `group` waves' pieces
-  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const Limits lim = row_limits(a, r);
-  Row<T, THR, NP> row;
-  row.init((const T*)a.score + (int64_t)r * a.ld, a.cols);
+// The cut at which the running sum of `value` over the order, `above` before the largest key, reaches the
+// target, among the elements that `in` admits.
+template <int THR, typename S, typename In, typename Value, typename Target>
+__device__ Cut find_cut(const S& src, Shared<THR>& sh, uint32_t kmin, uint32_t kmax, uint64_t above, int cols, In in,
+                        Value value, Target target_of) {
+  const Place p = descend<THR>(
+      sh, kmin, kmax, above,
+      [&](auto f) {
+        src.each([&](uint32_t k, int i) {
+          if (in(k, i)) f(k, [&] { return value(k); });
+        });
+      },
+      target_of);
+  // one key left: its elements each add the same; the lowest indices are kept
+  const uint64_t one = value(p.key), need = one ? (p.target - p.above + one - 1) / one : 1, have = one ? p.sum / one : 1;
+  if (need >= have) return Cut{p.key, 0x7fffffff};
+  const Place q = descend<THR>(
+      sh, ALL - (uint32_t)(cols - 1), ALL, 0,
+      [&](auto f) {
+        src.each([&](uint32_t k, int i) {
+          if (k == p.key && in(k, i)) f(ALL - (uint32_t)i, [] { return (uint64_t)1; });
+        });
+      },
+      [&](uint64_t) { return need; });
+  return Cut{p.key, (int)(ALL - q.key)};
+}
 
-  uint32_t kmax = 0, kmin = ALL;
-  row.each([&](int, int, const uint32_t* k) {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      kmax = max(kmax, k[e]);
-      kmin = min(kmin, k[e] ? k[e] : ALL);
-    }
-  });
+__device__ __forceinline__ uint64_t count_target(const Limits& l, uint64_t total) { return min((uint64_t)l.top_k, total); }
+__device__ __forceinline__ uint64_t weight_target(const Limits& l, uint64_t total) {
+  const double t = ceil(l.top_p * (double)total);
+  return t < 1.0 ? (uint64_t)1 : min(total, (uint64_t)t);
+}
+
+// The number in [0, sum) that the drawn u stands for; NaN and negative u: 0.
+__device__ __forceinline__ uint64_t draw_at(const RowArgs& a, int64_t at, uint64_t sum) {
+  const double u = a.u_wide ? ((const double*)a.u)[at] : (double)((const float*)a.u)[at];
+  const double x = u > 0.0 ? u * (double)sum : 0.0;
+  return x < (double)sum ? min((uint64_t)x, sum - 1) : sum - 1;
+}
+__device__ __forceinline__ double log_of_sum(uint64_t sum, const Limits& l) {
+  return log((double)sum) - (double)l.shift * 0.69314718055994530942;
+}
+__device__ __forceinline__ void store_draw(const RowArgs& a, int64_t at, int id, uint32_t key, const Limits& l, double log_sum) {
+  a.ids[at] = id;
+  if (a.logp) a.logp[at] = (float)((key == l.kmax ? 0.0 : ((double)key_score(key) - l.top) * l.inv_t) - log_sum);
+}
+__device__ __forceinline__ void store_none(const RowArgs& a, int64_t at) {
+  a.ids[at] = -1;
+  if (a.logp) a.logp[at] = -__builtin_inff();
+}
+
+// Largest and smallest key (0: none) over the workgroup.
+template <int THR>
+__device__ __forceinline__ void block_minmax(Shared<THR>& sh, uint32_t& kmax, uint32_t& kmin) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     kmax = max(kmax, __shfl_xor(kmax, o));
     kmin = min(kmin, __shfl_xor(kmin, o));
   }
-  if (lane == 0) {
-    sh.kmax[w] = kmax;
-    sh.kmin[w] = kmin;
+  if ((threadIdx.x & 63) == 0) {
+    sh.kmax[threadIdx.x >> 6] = kmax;
+    sh.kmin[threadIdx.x >> 6] = kmin;
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < WAVES; ++u) {
+  for (int u = 0; u < THR / WAVE; ++u) {
     kmax = max(kmax, sh.kmax[u]);
     kmin = min(kmin, sh.kmin[u]);
   }
+}
+
+template <typename T, int THR, int KEYS>
+__global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
+  constexpr int VE = Row<T, THR, KEYS>::VE, WAVES = THR / WAVE;
+  __shared__ __align__(16) uint32_t keys[KEYS > 0 ? KEYS : 4];
+  const int subs = (a.cols + WAVE * VE - 1) / (WAVE * VE);  // a wave's pieces: WAVE * VE consecutive scores
+  const int group = (subs + CHUNKS - 1) / CHUNKS, chunks = (subs + group - 1) / group;
+  __shared__ Shared<THR> sh;
+  extern __shared__ uint64_t chunk[];  // running kept weight after each chunk of `group` waves' pieces
+  const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  Limits lim = row_limits(a, r);
+  Row<T, THR, KEYS> row;
+  row.init((const T*)a.score + (int64_t)r * a.ld, a.cols, keys);
+
+  uint32_t kmax = 0, kmin = ALL;
+  row.each([&](uint32_t k, int) {
+    kmax = max(kmax, k);
+    kmin = min(kmin, k);
+  });
+  block_minmax(sh, kmax, kmin);
   if (kmax == 0) {  // nothing to take
-    for (int d = threadIdx.x; d < a.draws; d += THR) {
-      a.ids[(int64_t)r * a.draws + d] = -1;
-      if (a.logp) a.logp[(int64_t)r * a.draws + d] = -__builtin_inff();
-    }
+    for (int d = threadIdx.x; d < a.draws; d += THR) store_none(a, (int64_t)r * a.draws + d);
     return;
   }
-  const float top = key_score(kmax);
+  set_top(lim, kmax);
 
   Cut cut{0, 0x7fffffff};
   if (lim.top_k != ALL)
-    cut = find_cut<Row<T, THR, NP>, THR>(
-        row, sh, kmin, kmax, [](uint32_t, int) { return true; }, [](uint32_t) { return (uint64_t)1; },
-        [&](uint64_t total) { return min((uint64_t)lim.top_k, total); });
+    cut = find_cut<THR>(
+        row, sh, kmin, kmax, 0, a.cols, [](uint32_t, int) { return true; }, [](uint32_t) { return (uint64_t)1; },
+        [&](uint64_t total) { return count_target(lim, total); });
   if (lim.top_p < 1.0) {
     const Cut first = cut;
-    cut = find_cut<Row<T, THR, NP>, THR>(
-        row, sh, max(kmin, first.key), kmax, [&](uint32_t k, int i) { return first.keeps(k, i); },
-        [&](uint32_t k) { return weight(k, top, lim); },
-        [&](uint64_t total) {
-          const double t = ceil(lim.top_p * (double)total);
-          return t < 1.0 ? (uint64_t)1 : min(total, (uint64_t)t);
-        });
+    cut = find_cut<THR>(
+        row, sh, max(kmin, first.key), kmax, 0, a.cols, [&](uint32_t k, int i) { return first.keeps(k, i); },
+        [&](uint32_t k) { return weight(k, lim); }, [&](uint64_t total) { return weight_target(lim, total); });
   }
 
   // running sums of the kept weights over chunks of consecutive scores
-  const auto kept = [&](uint32_t k, int i) -> uint64_t {
-    if (!k || !cut.keeps(k, i)) return 0;
-    if (lim.min_p > 0) {
-      double v;
-      const uint64_t x = weight(k, top, lim, &v);
-      return v >= lim.min_p || k == kmax ? x : 0;
-    }
-    return weight(k, top, lim);
-  };
   for (int c = threadIdx.x; c < chunks; c += THR) chunk[c] = 0;
   __syncthreads();
-  row.each([&](int q, int i0, const uint32_t* k) {
+  row.pieces_of([&](int q, int i0, const uint32_t* k) {
     uint64_t s = 0;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s += kept(k[e], i0 + e);
+    for (int e = 0; e < VE; ++e) s += kept_weight(k[e], i0 + e, cut, lim);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       const uint32_t lo = __shfl_xor((uint32_t)s, o), hi = __shfl_xor((uint32_t)(s >> 32), o);
@@ -373,29 +449,25 @@ __global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
   __syncthreads();
 
   // a wave a draw: the first chunk whose running sum exceeds u * sum, then the score within it
-  const double log_sum = a.logp ? log((double)sum) - (double)lim.shift * 0.69314718055994530942 : 0.0;
+  const double log_sum = a.logp ? log_of_sum(sum, lim) : 0.0;
   for (int d = w; d < a.draws; d += WAVES) {
     const int64_t at = (int64_t)r * a.draws + d;
-    const double u = a.u_wide ? ((const double*)a.u)[at] : (double)((const float*)a.u)[at];
-    const double x = u > 0.0 ? u * (double)sum : 0.0;  // NaN: 0
-    const uint64_t t = x < (double)sum ? min((uint64_t)x, sum - 1) : sum - 1;
+    const uint64_t t = draw_at(a, at, sum);
     int lo = 0, hi = chunks - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (chunk[mid] > t) hi = mid;
       else lo = mid + 1;
     }
-    uint64_t run = lo ? chunk[lo - 1] : 0;
-    float s[VE];
-    uint64_t wt[VE];
+    uint64_t run = lo ? chunk[lo - 1] : 0, wt[VE];
+    uint32_t k[VE];
     int i0, who;
     for (int sub = lo * group;; ++sub) {  // the chunk's pieces in order; one of them passes t
       i0 = (sub * WAVE + lane) * VE;
-      const int m = a.cols - i0;
       uint64_t own = 0;
-      if (m > 0) load_piece<T>(s, row.p + i0, m);
+      row.read_at(i0, k);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) own += wt[e] = e < m ? kept(score_key(s[e]), i0 + e) : 0;
+      for (int e = 0; e < VE; ++e) own += wt[e] = kept_weight(k[e], i0 + e, cut, lim);
       const uint64_t end = run + wave_scan64(own);
       const uint64_t past = __ballot(end > t);
       if (past || sub + 1 >= min(subs, (lo + 1) * group)) {
@@ -406,38 +478,30 @@ __global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
       run = shfl64(end, WAVE - 1);
     }
     if (lane == who) {
-      int id = -1;
-      float sc = top;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
+        if (run <= t && run + wt[e] > t) store_draw(a, at, i0 + e, k[e], lim, log_sum);
         run += wt[e];
-        if (id < 0 && run > t) {
-          id = i0 + e;
-          sc = s[e];
-        }
       }
-      a.ids[at] = id;
-      if (a.logp) a.logp[at] = (float)((sc == top ? 0.0 : ((double)sc - (double)top) * lim.inv_t) - log_sum);
     }
   }
 }
 
-template <typename T, int THR, int NP>
+template <typename T, int THR, int KEYS>
 int launch(const RowArgs& a, hipStream_t st) {
-  const size_t lds = (size_t)std::min((a.cols + WAVE * Piece<T>::VE - 1) / (WAVE * Piece<T>::VE) + 1, CHUNKS) * 8;
-  k_sample<T, THR, NP><<<a.rows, THR, lds, st>>>(a);
+  constexpr int piece = WAVE * Row<T, THR, KEYS>::VE;
+  const size_t lds = (size_t)std::min((a.cols + piece - 1) / piece, CHUNKS) * 8;
+  k_sample<T, THR, KEYS><<<a.rows, THR, lds, st>>>(a);
   return check_launch("sample");
 }
 
 template <typename T>
 int dispatch(const RowArgs& a, hipStream_t st) {
-  constexpr int VE = Piece<T>::VE;
-  if (a.cols <= 256 * MAX_KEYS / 4) return launch<T, 256, 8 / VE>(a, st);
-  const int np = (a.cols + 1024 * VE - 1) / (1024 * VE);
-  if (np <= 8 / VE) return launch<T, 1024, 8 / VE>(a, st);
-  if (np <= 16 / VE) return launch<T, 1024, 16 / VE>(a, st);
-  if (np <= 24 / VE) return launch<T, 1024, 24 / VE>(a, st);
-  if (np <= 32 / VE) return launch<T, 1024, 32 / VE>(a, st);
+  if (a.cols <= 2048) return launch<T, 256, 2048>(a, st);
+  if (a.cols <= 8192) return launch<T, 512, 8192>(a, st);
+  if (a.cols <= 16384) return launch<T, 1024, 16384>(a, st);
+  if (a.cols <= 24576) return launch<T, 1024, 24576>(a, st);
+  if (a.cols <= ROW_KEYS) return launch<T, 1024, ROW_KEYS>(a, st);
   return launch<T, 1024, 0>(a, st);
 }
 
@@ -472,7 +536,7 @@ int sample(const regcn_sample_desc& d, hipStream_t st) {
   a.logp = d.logp;
   int bits = 0;
   while ((1ll << bits) < d.cols) ++bits;
-  a.shift = std::min(52, 63 - bits);
+  a.shift = std::min(51, 63 - bits);
   if (d.dtype == REGCN_F32) return dispatch<float>(a, st);
   if (d.dtype == REGCN_BF16) return dispatch<__bf16>(a, st);
   return dispatch<_Float16>(a, st);

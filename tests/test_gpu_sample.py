@@ -1,7 +1,7 @@
 """Sampling (csrc/sample.hip, ranking.sample) against a plain 64-bit restatement on the host.
 
 Ids are whole numbers and have to be equal.  The kernel's weights are exact multiples of 2^-S,
-S = min(52, 63 - ceil(log2 N)), the restatement's are doubles: a border is off by at most N 2^-(S+1)
+S = min(51, 63 - ceil(log2 N)), the restatement's are doubles: a border is off by at most N 2^-(S+1)
 of the largest weight (2^-33 at N = 2^15), so a draw lands between the two borders of one id with
 probability below N times that: under 1e-5 for the largest case here; the numbers are fixed by their seeds.
 The log-probability is (s - max) / T - log(sum), rounded once to fp32; sum is off by at most N 2^-(S+1)
