@@ -30,8 +30,15 @@ namespace {
 constexpr int HBITS = 11, HBINS = 1 << HBITS;
 constexpr int ROW_KEYS = 32768;  // scores of a row held in LDS
 constexpr uint32_t ALL = 0xffffffffu;
+constexpr int LIST = 256;        // members of a bin that are put in order one against the other
 constexpr int CHUNKS = 4096;  // running sums of kept weights kept in LDS, at most
 constexpr int MAX_COLS = 1 << 24;
+
+// Constants of scaled_exp, as kernel arguments: in scalar registers each is an operand of its fma (as literals
+// the compiler copies every one into vector registers first, a third of the instructions).
+struct ExpConsts {
+  double log2e, round, ln2_hi, ln2_lo, p[11];  // p: 1 / 12!, ..., 1 / 2!
+};
 
 struct RowArgs {
   const void* score;
@@ -44,6 +51,7 @@ struct RowArgs {
   const int32_t* top_k_v;
   int64_t* ids;
   float* logp;
+  ExpConsts c;
 };
 
 struct Limits {
@@ -54,6 +62,7 @@ struct Limits {
   uint32_t kmax;
   double top;
   bool ties_only;  // an infinite score, or a temperature whose inverse is: weight only on the largest
+  ExpConsts c;
 };
 
 __device__ __forceinline__ Limits row_limits(const RowArgs& a, int row) {
@@ -69,6 +78,7 @@ __device__ __forceinline__ Limits row_limits(const RowArgs& a, int row) {
     l.top_k = 1;
   }
   l.shift = a.shift;
+  l.c = a.c;
   return l;
 }
 
@@ -87,26 +97,22 @@ __device__ __forceinline__ void set_top(Limits& l, uint32_t kmax) {
 }
 
 // exp(x) 2^S for x = (s - top) / T <= 0.  exp(x) = 2^n p(r), r = x - n ln 2 in two parts, |r| <= ln 2 / 2;
-// p is the Taylor polynomial of degree 12 (remainder below 2^-52 of p).
+// p is the Taylor polynomial of degree 12 (remainder below 2^-52 of p).  n comes out of the low bits of
+// x / ln 2 + 1.5 2^52 and goes into the exponent of p by an integer add (n + S >= -1010: still normal): the
+// conversions, rounding and ldexp instructions run at a quarter of the rate of the rest.
 __device__ __forceinline__ double scaled_exp(uint32_t key, const Limits& l) {
   const double x = fmax(((double)key_score(key) - l.top) * l.inv_t, -700.0);
-  const double n = __builtin_rint(x * 1.4426950408889634074);
-  double r = fma(n, -6.93147180369123816490e-01, x);
-  r = fma(n, -1.90821492927058770002e-10, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
+  const double t = fma(x, l.c.log2e, l.c.round);
+  const double n = t - l.c.round;
+  double r = fma(n, l.c.ln2_hi, x);
+  r = fma(n, l.c.ln2_lo, r);
+  double p = fma(l.c.p[0], r, l.c.p[1]);
+#pragma unroll
+  for (int j = 2; j < 11; ++j) p = fma(p, r, l.c.p[j]);
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
-  return __builtin_ldexp(p, (int)n + l.shift);
+  const int e = (int)(uint32_t)__double_as_longlong(t) + l.shift;
+  return __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
 }
 
 // To the nearest whole number: adding 2^52 to a number up to 2^51 leaves it in the low bits.
@@ -124,12 +130,46 @@ struct Cut {
   __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= idx); }
 };
 
-// The weight of an element, 0 where a limit leaves it out.
-__device__ __forceinline__ uint64_t kept_weight(uint32_t key, int idx, const Cut& cut, const Limits& l) {
-  if (!key || !cut.keeps(key, idx)) return 0;
-  if (l.ties_only) return key == l.kmax ? 1ull << l.shift : 0;
-  const double v = scaled_exp(key, l);
-  return v >= l.min_w || key == l.kmax ? whole(v) : 0;
+// The weights of a piece's elements, 0 where a limit leaves one out.  No branch an element: the exponentials
+// of the piece run together, and pieces without an element kept by any lane are passed over.
+template <int VE>
+__device__ __forceinline__ void kept_weights(const uint32_t* k, int i0, const Cut& cut, const Limits& l, uint64_t (&w)[VE]) {
+  bool keep[VE], some = false;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    keep[e] = k[e] && cut.keeps(k[e], i0 + e);
+    some |= keep[e];
+    w[e] = 0;
+  }
+  if (!some) return;
+  if (l.ties_only) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) w[e] = keep[e] && k[e] == l.kmax ? 1ull << l.shift : 0;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const double v = scaled_exp(k[e], l);
+    w[e] = keep[e] && (v >= l.min_w || k[e] == l.kmax) ? whole(v) : 0;
+  }
+}
+
+// Sum over the wave, in every lane: two halves by DPP within rows of 16 lanes, the four rows by readlane.
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+#define REGCN_STEP(ctrl)                                                                                       \
+  v += (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, ctrl, 0xF, 0xF, false) |            \
+       (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), ctrl, 0xF, 0xF, false) << 32
+  REGCN_STEP(0xB1);   // quad_perm [1,0,3,2]
+  REGCN_STEP(0x4E);   // quad_perm [2,3,0,1]
+  REGCN_STEP(0x124);  // row_ror:4
+  REGCN_STEP(0x128);  // row_ror:8
+#undef REGCN_STEP
+  uint64_t s = 0;
+#pragma unroll
+  for (int row = 0; row < 4; ++row)
+    s += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 16 * row) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 16 * row) << 32;
+  return s;
 }
 
 template <int THR>
@@ -138,7 +178,10 @@ struct Shared {
   uint64_t wave[THR / WAVE];
   uint32_t kmax[THR / WAVE], kmin[THR / WAVE];
   uint64_t above, sum;
-  uint32_t bin;
+  uint32_t bin, count, lo, hi;
+  uint2 list[LIST];      // {key, index}
+  uint64_t value[LIST];
+  Cut cut;
 };
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
@@ -205,22 +248,53 @@ struct Row {
       load(i0, k);
     }
   }
-  __device__ __forceinline__ void init(const T* row, int cols, uint32_t* lds) {
+  // Also the largest and smallest key (0, ALL: none) of this thread's.
+  __device__ __forceinline__ void init(const T* row, int cols, uint32_t* lds, uint32_t& kmax, uint32_t& kmin) {
+    kmax = 0;
+    kmin = ALL;
     p = row;
     n = cols;
     keys = lds;
     pieces = (cols + THR * VE - 1) / (THR * VE);
     if constexpr (KEYS > 0) {
-      constexpr int PV = Piece<T>::VE;
-#pragma unroll 8
-      for (int i0 = (int)threadIdx.x * PV; i0 < pieces * THR * VE; i0 += THR * PV) {
+      // all the row's loads under way at once: a loop over bounds-checked pieces waits for each
+      constexpr int PV = Piece<T>::VE, MOST = (KEYS + THR * PV - 1) / (THR * PV);
+      typedef typename Piece<T>::vec vec;
+      typedef typename Piece<T>::uvec uvec;
+      vec x[MOST];
+#pragma unroll
+      for (int q = 0; q < MOST; ++q) {
+        const int i0 = (q * THR + (int)threadIdx.x) * PV;
+        if (i0 + PV <= n) x[q] = *reinterpret_cast<const uvec*>(p + i0);
+      }
+#pragma unroll
+      for (int q = 0; q < MOST; ++q) {
+        const int i0 = (q * THR + (int)threadIdx.x) * PV;
+        if (i0 >= pieces * THR * VE) continue;
         uint32_t k[PV];
-        load(i0, k);
+        if (i0 + PV <= n) {
+#pragma unroll
+          for (int e = 0; e < PV; ++e) k[e] = score_key(to_f32<T>(x[q][e]));
+        } else {
+          load(i0, k);
+        }
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+          kmax = max(kmax, k[e]);
+          kmin = min(kmin, k[e] ? k[e] : ALL);
+        }
 #pragma unroll
         for (int e = 0; e < PV; e += 4)
           *reinterpret_cast<uint4*>(keys + i0 + e) = make_uint4(k[e], k[e + 1], k[e + 2], k[e + 3]);
       }
-      __syncthreads();
+    } else {
+      pieces_of([&](int, int, const uint32_t* k) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          kmax = max(kmax, k[e]);
+          kmin = min(kmin, k[e] ? k[e] : ALL);
+        }
+      });
     }
   }
   // f(q, first index, keys of the piece) for every piece
@@ -232,26 +306,6 @@ struct Row {
       read_at(i0, k);
       f(q, i0, k);
     }
-  }
-  // f(key, index) for every element
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    pieces_of([&](int, int i0, const uint32_t* k) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (k[e]) f(k[e], i0 + e);
-    });
-  }
-};
-
-// Elements in a list, in no order.
-template <int THR>
-struct List {
-  const uint2* p;
-  int n;
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x; i < n; i += THR) f(p[i].x, (int)p[i].y);
   }
 };
 
@@ -284,8 +338,8 @@ struct Place {
   uint64_t above, sum, target;  // sums before the key, of the key
 };
 
-// Radix descent in decreasing order of mapped keys in [lo, hi]: the key at which the running sum of values,
-// starting from `above`, reaches the target.  each(f) calls f(mapped key, value functor) for the elements.
+// Radix descent in decreasing order of keys in [lo, hi]: the key at which the running sum of values, `above`
+// before hi, reaches the target.  each(f, lo, hi) calls f(key, value) for the elements with a key in [lo, hi].
 template <int THR, typename Each, typename Target>
 __device__ Place descend(Shared<THR>& sh, uint32_t lo, uint32_t hi, uint64_t above, Each each, Target target_of) {
   uint64_t target = 0;
@@ -295,10 +349,9 @@ __device__ Place descend(Shared<THR>& sh, uint32_t lo, uint32_t hi, uint64_t abo
     const int shift = bits > HBITS ? bits - HBITS : 0;
     for (int b = threadIdx.x; b < HBINS; b += THR) sh.hist[b] = 0;
     __syncthreads();
-    each([&](uint32_t k, auto value) {
-      if (k >= lo && k <= hi)
-        atomicAdd((unsigned long long*)&sh.hist[(hi - k) >> shift], (unsigned long long)value());
-    });
+    each([&](uint32_t k, uint64_t value) {
+      if (value) atomicAdd((unsigned long long*)&sh.hist[(hi - k) >> shift], (unsigned long long)value);
+    }, lo, hi);
     __syncthreads();
     const uint64_t t = find_bin<THR, HBINS>(sh, sh.hist, above, [&](uint64_t total) { return first ? target_of(total) : target; });
     target = t;
@@ -313,27 +366,117 @@ __device__ Place descend(Shared<THR>& sh, uint32_t lo, uint32_t hi, uint64_t abo
   return p;
 }
 
-// The cut at which the running sum of `value` over the order, `above` before the largest key, reaches the
-// target, among the elements that `in` admits.
-template <int THR, typename S, typename In, typename Value, typename Target>
-__device__ Cut find_cut(const S& src, Shared<THR>& sh, uint32_t kmin, uint32_t kmax, uint64_t above, int cols, In in,
-                        Value value, Target target_of) {
+// The bin of a key's score on a linear scale from the largest score down (fp32: monotone, which is all that a
+// bin has to be); the last bin is open.
+__device__ __forceinline__ uint32_t value_bin(uint32_t key, float top, float per) {
+  return (uint32_t)fminf((top - key_score(key)) * per, (float)(HBINS - 1));
+}
+
+// The cut at which a running sum over the order reaches the target, among the elements that `from` keeps: of
+// ones (WEIGHTS false) or of weights.  First over 2048 bins of the scores' range, at most 44 T of it (weights
+// below exp(-44) are none): the bin in question then rarely has over LIST members, and each of those adds up
+// the members before it.  Otherwise, and for infinite scores, a descent over the keys.
+template <bool WEIGHTS, int THR, typename R, typename Target>
+__device__ Cut find_cut(const R& row, Shared<THR>& sh, uint32_t kmin, uint32_t kmax, int cols, const Cut& from,
+                        const Limits& lim, Target target_of) {
+  constexpr int VE = R::VE;
+  uint64_t above = 0, target = 0;
+  const float top = key_score(kmax), span = fminf(top - key_score(kmin), (float)(44.0 / lim.inv_t));
+  const float per = (float)HBINS / span;
+  if (per > 0.f && per < 1e30f && !lim.ties_only) {
+    for (int b = threadIdx.x; b < HBINS; b += THR) sh.hist[b] = 0;
+    if (threadIdx.x == 0) {
+      sh.count = 0;
+      sh.lo = ALL;
+      sh.hi = 0;
+    }
+    __syncthreads();
+    row.pieces_of([&](int, int i0, const uint32_t* k) {
+      uint64_t w[VE];
+      if (WEIGHTS) {
+        kept_weights<VE>(k, i0, from, lim, w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) w[e] = k[e] != 0;
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (w[e]) atomicAdd((unsigned long long*)&sh.hist[value_bin(k[e], top, per)], (unsigned long long)w[e]);
+    });
+    __syncthreads();
+    target = find_bin<THR, HBINS>(sh, sh.hist, 0, target_of);
+    above = sh.above;
+    const uint32_t bin = sh.bin;
+    row.pieces_of([&](int, int i0, const uint32_t* k) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (k[e] && value_bin(k[e], top, per) == bin && from.keeps(k[e], i0 + e)) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < LIST) sh.list[at] = make_uint2(k[e], (uint32_t)(i0 + e));
+          atomicMin(&sh.lo, k[e]);
+          atomicMax(&sh.hi, k[e]);
+        }
+    });
+    __syncthreads();
+    const int count = (int)sh.count;
+    if (count <= LIST) {
+      uint2 me = make_uint2(0, 0);
+      uint64_t own = 0, before = above;
+      if ((int)threadIdx.x < count) {
+        me = sh.list[threadIdx.x];
+        own = WEIGHTS ? weight(me.x, lim) : 1;
+        sh.value[threadIdx.x] = own;
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < count) {
+#pragma unroll 4
+        for (int j = 0; j < count; ++j) {
+          const uint2 o = sh.list[j];
+          before += o.x > me.x || (o.x == me.x && o.y < me.y) ? sh.value[j] : 0;
+        }
+        if (before < target && before + own >= target) sh.cut = Cut{me.x, (int)me.y};  // one thread's
+      }
+      __syncthreads();
+      const Cut cut = sh.cut;
+      __syncthreads();  // sh may be written again
+      return cut;
+    }
+    kmin = sh.lo;
+    kmax = sh.hi;
+    __syncthreads();
+  }
   const Place p = descend<THR>(
       sh, kmin, kmax, above,
-      [&](auto f) {
-        src.each([&](uint32_t k, int i) {
-          if (in(k, i)) f(k, [&] { return value(k); });
+      [&](auto f, uint32_t lo, uint32_t hi) {
+        row.pieces_of([&](int, int i0, const uint32_t* k) {
+          uint64_t w[VE];
+          if (WEIGHTS) {
+            uint32_t in[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) in[e] = k[e] >= lo && k[e] <= hi ? k[e] : 0;
+            kept_weights<VE>(in, i0, from, lim, w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) w[e] = k[e] && k[e] >= lo && k[e] <= hi;
+          }
+#pragma unroll
+          for (int e = 0; e < VE; ++e) f(k[e], w[e]);
         });
       },
-      target_of);
+      [&](uint64_t total) { return target ? target : target_of(total); });
   // one key left: its elements each add the same; the lowest indices are kept
-  const uint64_t one = value(p.key), need = one ? (p.target - p.above + one - 1) / one : 1, have = one ? p.sum / one : 1;
+  const uint64_t one = WEIGHTS ? weight(p.key, lim) : 1;
+  const uint64_t need = one ? (p.target - p.above + one - 1) / one : 1, have = one ? p.sum / one : 1;
   if (need >= have) return Cut{p.key, 0x7fffffff};
   const Place q = descend<THR>(
       sh, ALL - (uint32_t)(cols - 1), ALL, 0,
-      [&](auto f) {
-        src.each([&](uint32_t k, int i) {
-          if (k == p.key && in(k, i)) f(ALL - (uint32_t)i, [] { return (uint64_t)1; });
+      [&](auto f, uint32_t lo, uint32_t hi) {
+        row.pieces_of([&](int, int i0, const uint32_t* k) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const uint32_t at = ALL - (uint32_t)(i0 + e);
+            f(at, k[e] == p.key && from.keeps(k[e], i0 + e) && at >= lo && at <= hi);
+          }
         });
       },
       [&](uint64_t) { return need; });
@@ -364,7 +507,7 @@ __device__ __forceinline__ void store_none(const RowArgs& a, int64_t at) {
   if (a.logp) a.logp[at] = -__builtin_inff();
 }
 
-// Largest and smallest key (0: none) over the workgroup.
+// Largest and smallest key (0, ALL: none) over the workgroup; a barrier.
 template <int THR>
 __device__ __forceinline__ void block_minmax(Shared<THR>& sh, uint32_t& kmax, uint32_t& kmin) {
 #pragma unroll
@@ -395,13 +538,8 @@ __global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
   const int r = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   Limits lim = row_limits(a, r);
   Row<T, THR, KEYS> row;
-  row.init((const T*)a.score + (int64_t)r * a.ld, a.cols, keys);
-
-  uint32_t kmax = 0, kmin = ALL;
-  row.each([&](uint32_t k, int) {
-    kmax = max(kmax, k);
-    kmin = min(kmin, k);
-  });
+  uint32_t kmax, kmin;
+  row.init((const T*)a.score + (int64_t)r * a.ld, a.cols, keys, kmax, kmin);
   block_minmax(sh, kmax, kmin);
   if (kmax == 0) {  // nothing to take
     for (int d = threadIdx.x; d < a.draws; d += THR) store_none(a, (int64_t)r * a.draws + d);
@@ -410,29 +548,24 @@ __global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
   set_top(lim, kmax);
 
   Cut cut{0, 0x7fffffff};
+  const double min_w = lim.min_w;
+  lim.min_w = 0;  // min_p looks at what the other two leave
   if (lim.top_k != ALL)
-    cut = find_cut<THR>(
-        row, sh, kmin, kmax, 0, a.cols, [](uint32_t, int) { return true; }, [](uint32_t) { return (uint64_t)1; },
-        [&](uint64_t total) { return count_target(lim, total); });
-  if (lim.top_p < 1.0) {
-    const Cut first = cut;
-    cut = find_cut<THR>(
-        row, sh, max(kmin, first.key), kmax, 0, a.cols, [&](uint32_t k, int i) { return first.keeps(k, i); },
-        [&](uint32_t k) { return weight(k, lim); }, [&](uint64_t total) { return weight_target(lim, total); });
-  }
+    cut = find_cut<false, THR>(row, sh, kmin, kmax, a.cols, cut, lim, [&](uint64_t total) { return count_target(lim, total); });
+  if (lim.top_p < 1.0)
+    cut = find_cut<true, THR>(row, sh, max(kmin, cut.key), kmax, a.cols, Cut(cut), lim,
+                              [&](uint64_t total) { return weight_target(lim, total); });
+  lim.min_w = min_w;
 
   // running sums of the kept weights over chunks of consecutive scores
   for (int c = threadIdx.x; c < chunks; c += THR) chunk[c] = 0;
   __syncthreads();
   row.pieces_of([&](int q, int i0, const uint32_t* k) {
-    uint64_t s = 0;
+    uint64_t wt[VE], s = 0;
+    kept_weights<VE>(k, i0, cut, lim, wt);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s += kept_weight(k[e], i0 + e, cut, lim);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint32_t lo = __shfl_xor((uint32_t)s, o), hi = __shfl_xor((uint32_t)(s >> 32), o);
-      s += (uint64_t)hi << 32 | lo;
-    }
+    for (int e = 0; e < VE; ++e) s += wt[e];
+    s = wave_sum64(s);
     const int sub = q * WAVES + w;
     if (lane == 0 && sub < subs) atomicAdd((unsigned long long*)&chunk[sub / group], (unsigned long long)s);
   });
@@ -466,8 +599,9 @@ __global__ __launch_bounds__(THR) void k_sample(RowArgs a) {
       i0 = (sub * WAVE + lane) * VE;
       uint64_t own = 0;
       row.read_at(i0, k);
+      kept_weights<VE>(k, i0, cut, lim, wt);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) own += wt[e] = kept_weight(k[e], i0 + e, cut, lim);
+      for (int e = 0; e < VE; ++e) own += wt[e];
       const uint64_t end = run + wave_scan64(own);
       const uint64_t past = __ballot(end > t);
       if (past || sub + 1 >= min(subs, (lo + 1) * group)) {
@@ -534,6 +668,12 @@ int sample(const regcn_sample_desc& d, hipStream_t st) {
   a.min_p_v = d.min_p_rows;
   a.ids = d.ids;
   a.logp = d.logp;
+  a.c.log2e = 1.4426950408889634074;
+  a.c.round = 0x1.8p52;
+  a.c.ln2_hi = -6.93147180369123816490e-01;
+  a.c.ln2_lo = -1.90821492927058770002e-10;
+  double f = 1.0;
+  for (int j = 2; j <= 12; ++j) a.c.p[12 - j] = 1.0 / (f *= j);
   int bits = 0;
   while ((1ll << bits) < d.cols) ++bits;
   a.shift = std::min(51, 63 - bits);
