@@ -590,6 +590,7 @@ struct Spread {
   uint64_t* seg_sum;  // rows x segs
   Member* list;       // rows x cap
   int segs, cap;
+  int per;  // segments a workgroup of the range, histogram and member launches
 };
 
 template <typename T>
@@ -616,9 +617,11 @@ __global__ __launch_bounds__(256) void k_spread_clear(Spread p) {
 
 template <typename T>
 __global__ __launch_bounds__(SEG_THR) void k_spread_range(Spread p) {
-  const int r = blockIdx.y, begin = blockIdx.x * SEG;
+  __shared__ uint32_t ends[2];
+  const int r = blockIdx.y, begin = blockIdx.x * p.per * SEG;
   uint32_t hi = 0, lo = 0;
-  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + SEG, p.a.cols), [&](const float* x, int) {
+  if (threadIdx.x < 2) ends[threadIdx.x] = 0;
+  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + p.per * SEG, p.a.cols), [&](const float* x, int) {
 #pragma unroll
     for (int e = 0; e < Piece<T>::VE; ++e)
       if (x[e] >= LOWEST) {
@@ -628,9 +631,15 @@ __global__ __launch_bounds__(SEG_THR) void k_spread_range(Spread p) {
   });
   hi = wave_max(hi);
   lo = wave_max(lo);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0 && hi) {
-    atomicMax(&p.state[r].kmax, hi);
-    atomicMax(&p.state[r].kmin_inv, lo);
+    atomicMax(&ends[0], hi);
+    atomicMax(&ends[1], lo);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && ends[0]) {
+    atomicMax(&p.state[r].kmax, ends[0]);
+    atomicMax(&p.state[r].kmin_inv, ends[1]);
   }
 }
 
@@ -652,14 +661,14 @@ __device__ __forceinline__ Cut cut_k(const Spread& p, int r, const Limits& l) {
 template <typename T, bool WEIGHTS>
 __global__ __launch_bounds__(SEG_THR) void k_spread_hist(Spread p) {
   __shared__ uint64_t hist[HBINS];
-  const int r = blockIdx.y, begin = blockIdx.x * SEG;
+  const int r = blockIdx.y, begin = blockIdx.x * p.per * SEG;
   Limits l;
   float per;
   if (!spread_limits<WEIGHTS>(p, r, l, per) || !bins_work(per, l)) return;
   const Cut from = WEIGHTS ? cut_k(p, r, l) : Cut{LOWEST, NO_TIE};
   for (int b = threadIdx.x; b < HBINS; b += SEG_THR) hist[b] = 0;
   __syncthreads();
-  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + SEG, p.a.cols), [&](const float* x, int i0) {
+  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + p.per * SEG, p.a.cols), [&](const float* x, int i0) {
     add_to_bins<WEIGHTS, Piece<T>::VE>(hist, x, i0, from, per, l, p.a.c);
   });
   __syncthreads();
@@ -671,7 +680,7 @@ __global__ __launch_bounds__(SEG_THR) void k_spread_hist(Spread p) {
 template <typename T, bool WEIGHTS>
 __global__ __launch_bounds__(SEG_THR) void k_spread_members(Spread p) {
   __shared__ Shared<SEG_THR> sh;
-  const int r = blockIdx.y, begin = blockIdx.x * SEG;
+  const int r = blockIdx.y, begin = blockIdx.x * p.per * SEG;
   Limits l;
   float per;
   if (!spread_limits<WEIGHTS>(p, r, l, per) || !bins_work(per, l)) return;
@@ -686,7 +695,7 @@ __global__ __launch_bounds__(SEG_THR) void k_spread_members(Spread p) {
     st.target[WEIGHTS] = target;
     st.ready[WEIGHTS] = 1;
   }
-  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + SEG, p.a.cols), [&](const float* x, int i0) {
+  each_piece<T, SEG_THR>(row_of<T>(p, r), p.a.cols, begin, min(begin + p.per * SEG, p.a.cols), [&](const float* x, int i0) {
     members<Piece<T>::VE>(x, i0, from, bin, per, l, [&](float s, int i) {
       const uint32_t at = atomicAdd(&st.count[WEIGHTS], 1u);
       if (at < (uint32_t)p.cap) p.list[(int64_t)r * p.cap + at] = Member{s, i};
@@ -850,7 +859,7 @@ int rows_at_once(int cols) {
 
 template <typename T, bool WEIGHTS>
 void launch_cut(const Spread& p, hipStream_t st) {
-  const dim3 grid(p.segs, p.a.rows);
+  const dim3 grid((p.segs + p.per - 1) / p.per, p.a.rows);
   k_spread_hist<T, WEIGHTS><<<grid, SEG_THR, 0, st>>>(p);
   k_spread_members<T, WEIGHTS><<<grid, SEG_THR, 0, st>>>(p);
   k_spread_cut<T, WEIGHTS><<<p.a.rows, 1024, 0, st>>>(p);
@@ -862,6 +871,9 @@ int launch_spread(const RowArgs& a, void* ws, hipStream_t st) {
   p.a = a;
   p.segs = (a.cols + SEG - 1) / SEG;
   p.cap = list_cap(a.cols);
+  // every workgroup adds its histogram to the row's by atomics on the same 2048 words: no more of them than
+  // fill the card twice (16 x 1 M: 53 us with a segment each, 20 with 4)
+  p.per = (int)std::max<int64_t>(1, std::min<int64_t>(16, (int64_t)a.rows * p.segs / 512));
   char* w = (char*)ws;
   p.state = (RowState*)w;
   w += round256((int64_t)a.rows * sizeof(RowState));
@@ -871,7 +883,7 @@ int launch_spread(const RowArgs& a, void* ws, hipStream_t st) {
   const int64_t words = (int64_t)a.rows * sizeof(RowState) / 8;
   k_spread_clear<<<(int)std::min<int64_t>((words + 255) / 256, 2048), 256, 0, st>>>(p);
   const dim3 grid(p.segs, a.rows);
-  k_spread_range<T><<<grid, SEG_THR, 0, st>>>(p);
+  k_spread_range<T><<<dim3((p.segs + p.per - 1) / p.per, a.rows), SEG_THR, 0, st>>>(p);
   if (a.top_k_v || (a.top_k > 0 && a.top_k < a.cols) || a.temperature_v || !(a.temperature > 0)) launch_cut<T, false>(p, st);
   if (a.top_p_v || a.top_p < 1.0) launch_cut<T, true>(p, st);
   k_spread_sums<T><<<grid, SEG_THR, 0, st>>>(p);
