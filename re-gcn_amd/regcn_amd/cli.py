@@ -32,9 +32,9 @@ import time
 import numpy as np
 import torch
 
-from . import ranking
+from . import muon, ranking
 from .graph import build_sub_graph
-from .training import GraphedSteps
+from .training import GraphedSteps, use_sorted_lookup
 from .weights import bump_versions, invalidate
 
 logger = logging.getLogger("regcn_amd.cli")
@@ -127,7 +127,49 @@ def build_parser():
       help="--test with several ranks (torchrun): partition every snapshot over the ranks (destination "
            "owners + all-gather, or edge slices + all-reduce) and the entity candidates of the decoder "
            "(SURVEY.md §8(e)); default: rank 0 evaluates alone")
+    a("--optimizer", type=str, default="adam", choices=["adam", "muon"],
+      help="muon: orthogonalised momentum (muon.Muon) for the two-dimensional weights, Adam for the tables, "
+           "vectors and scalars")
+    a("--muon-lr", type=float, default=0.02)
+    a("--muon-momentum", type=float, default=0.95)
+    a("--sorted-lookup", action="store_true",
+      help="training: the decoders look rows up through autograd.embedding, whose gradient sums each row's "
+           "triples in a fixed order without atomics")
+    a("--sample-draws", type=int, default=0,
+      help="--multi-step: draw this many answers a query from its scores for the next history instead of taking "
+           "the --topk best (0); the four limits below shape the draw")
+    a("--sample-temperature", type=float, default=1.0)
+    a("--sample-top-k", type=int, default=0)
+    a("--sample-top-p", type=float, default=1.0)
+    a("--sample-min-p", type=float, default=0.0)
     return p
+
+
+class Optimizers:
+    """Several optimizers over disjoint parameters as one."""
+
+    def __init__(self, *optimizers):
+        self.optimizers = optimizers
+
+    def zero_grad(self):
+        for o in self.optimizers:
+            o.zero_grad()
+
+    def step(self):
+        for o in self.optimizers:
+            o.step()
+
+
+def _next_snap(args, test_triples, num_nodes, num_rels, score, score_r):
+    """The --multi-step history's next snapshot from the scores of this one."""
+    rel = args.relation_evaluation
+    if getattr(args, "sample_draws", 0):
+        return ranking.construct_snap_sampled(
+            test_triples, num_nodes, num_rels, score_r if rel else score, args.sample_draws, relation=rel,
+            temperature=args.sample_temperature, top_k=args.sample_top_k, top_p=args.sample_top_p,
+            min_p=args.sample_min_p)
+    make, s = (ranking.construct_snap_r, score_r) if rel else (ranking.construct_snap, score)
+    return make(test_triples, num_nodes, num_rels, s, args.topk)
 
 
 def _unsupported(args):
@@ -251,9 +293,7 @@ def test(model, history_list, test_list, num_rels, num_nodes, device, all_ans_li
             if args.multi_step and score is None:
                 raise SystemExit("--multi-step builds the next history from the full score matrix: not with --shard")
             if args.multi_step:
-                pred = (ranking.construct_snap_r(test_triples, num_nodes, num_rels, score_r, args.topk)
-                        if args.relation_evaluation else
-                        ranking.construct_snap(test_triples, num_nodes, num_rels, score, args.topk))
+                pred = _next_snap(args, test_triples, num_nodes, num_rels, score, score_r)
                 if len(pred):
                     input_list.pop(0)
                     input_list.append(pred)
@@ -295,8 +335,14 @@ def train_model(args, model, train_list, valid, num_nodes, num_rels, device, mod
     # :469; the fused multi-tensor kernel: a handful of launches per step instead of ~100 (it
     # does not bump the parameters' version counters: bump_versions after each step)
     fused = device.type == "cuda"
-    optimizer = torch.optim.Adam(model.parameters(), lr=args.lr, weight_decay=1e-5,
-                                 capturable=graphed is not None, fused=fused)
+    adam = dict(lr=args.lr, weight_decay=1e-5, capturable=graphed is not None, fused=fused)
+    if args.optimizer == "muon":
+        mats, rest = muon.split_parameters(model)
+        optimizer = Optimizers(muon.Muon(mats, lr=args.muon_lr, momentum=args.muon_momentum, weight_decay=1e-5),
+                               torch.optim.Adam(rest, **adam))
+    else:
+        optimizer = torch.optim.Adam(model.parameters(), **adam)
+    use_sorted_lookup(model, args.sorted_lookup)
     # replicas: every rank takes its share of the shuffled samples, one gradient
     # all-reduce per optimizer step; the same seed on every rank keeps the shuffles (and so the
     # lock-step schedule) identical.  Rank 0 validates and checkpoints.
@@ -440,6 +486,8 @@ def main(argv=None):
         raise ValueError("--radius-msg-gamma must be non-negative (use 0 to disable the penalty)")
     if not 0.0 <= args.radius_anchor_beta <= 1.0:
         raise ValueError("--radius-anchor-beta must be in [0, 1]")
+    if args.sample_draws < 0:
+        raise ValueError("--sample-draws must be non-negative (0: the --topk best)")
     if args.gpu < 0 or not torch.cuda.is_available():
         raise SystemExit("the HIP path needs a GPU (--gpu N); there is no CPU fallback")
     world = int(os.environ.get("WORLD_SIZE", "1"))

@@ -148,8 +148,16 @@ def givens_reflection(x, angles):
     return torch.stack([co * x1 + si * x2, si * x1 - co * x2], dim=2).reshape(x.shape[0], x.shape[1])
 
 
+def _take(decoder, table, idx):
+    """table[idx]; with `sorted_lookup` (training.use_sorted_lookup) through autograd.embedding, whose
+    gradient sums each row's triples in a fixed order without atomics."""
+    return _ag.embedding(table, idx) if decoder.sorted_lookup else table[idx]
+
+
 class _EntityDecoderBase(nn.Module):
     """Shared state of MuRP/RotH/AttH entity decoders (hyperbolic_decoder.py:662-731)."""
+
+    sorted_lookup = False
 
     def _init_common(self, num_entities, num_relations, embedding_dim, c, dropout, query_chunk_size,
                      candidate_chunk_size, score_scale_init, score_margin_init, use_entity_euclidean_bias,
@@ -235,9 +243,9 @@ class HyperbolicMuRP(_EntityDecoderBase):
         """hyperbolic_decoder.py:745-764."""
         c = self.c
         r_idx = trip[:, 1]
-        s_emb = HyperbolicOps.project_to_ball(ent[trip[:, 0]], c)
+        s_emb = HyperbolicOps.project_to_ball(_take(self, ent, trip[:, 0]), c)
         s_tan = self.dropout(HyperbolicOps.log_map_zero(s_emb, c))
-        rr = rel[r_idx]
+        rr = _take(self, rel, r_idx)
         rot_s = HyperbolicOps.exp_map_zero((_ag.linear(self.rot_proj, rr) * s_tan).contiguous(), c)
         t_r = HyperbolicOps.exp_map_zero(_ag.linear(self.trans_proj, rr).contiguous(), c)
         return HyperbolicOps.mobius_add(HyperbolicOps.project_to_ball(rot_s, c),
@@ -289,9 +297,9 @@ class HyperbolicRotH(_EntityDecoderBase):
             return q
         c = self.c
         r_idx = trip[:, 1]
-        s_emb = HyperbolicOps.project_to_ball(ent[trip[:, 0]], c)
+        s_emb = HyperbolicOps.project_to_ball(_take(self, ent, trip[:, 0]), c)
         s_tan = self._reshape_tangent(self.dropout(HyperbolicOps.log_map_zero(s_emb, c)))
-        rr = rel[r_idx]  # one gather (and one index backward) for both projections
+        rr = _take(self, rel, r_idx)  # one gather (and one index backward) for both projections
         rot_s = HyperbolicOps.exp_map_zero(givens_rotation(s_tan, _ag.linear(self.rot_proj, rr)).contiguous(), c)
         t_r = HyperbolicOps.exp_map_zero(_ag.linear(self.trans_proj, rr).contiguous(), c)
         return HyperbolicOps.mobius_add(HyperbolicOps.project_to_ball(rot_s, c),
@@ -327,9 +335,9 @@ class HyperbolicAttH(_EntityDecoderBase):
         """hyperbolic_decoder.py:1414-1448."""
         c = self.c
         r_idx = trip[:, 1]
-        s_emb = HyperbolicOps.project_to_ball(ent[trip[:, 0]], c)
+        s_emb = HyperbolicOps.project_to_ball(_take(self, ent, trip[:, 0]), c)
         s_tan = self.dropout(HyperbolicOps.log_map_zero(s_emb, c))
-        rr = rel[r_idx]
+        rr = _take(self, rel, r_idx)
         rot_s = givens_rotation(s_tan, _ag.linear(self.rot_proj, rr))
         ref_s = givens_reflection(s_tan, _ag.linear(self.ref_proj, rr))
         a_r = torch.sigmoid(torch.sum(_ag.linear(self.attn_proj, rr) * torch.cat([s_tan, rr], dim=-1), dim=-1, keepdim=True))
@@ -414,6 +422,8 @@ def roth_pair_predict(dec, rdec, ent, rel, test_triplets, num_rels, parts=None):
 
 
 class _RelDecoderBase(nn.Module):
+    sorted_lookup = False
+
     def _score_scale(self):
         return F.softplus(self.score_scale_raw) + SCORE_SCALE_EPSILON
 
@@ -454,8 +464,8 @@ class HyperbolicMuRPRel(_RelDecoderBase):
 
     def _query(self, ent, trip):
         c = self.c
-        s_tan = self.dropout(HyperbolicOps.log_map_zero(ent[trip[:, 0]], c))
-        o_tan = self.dropout(HyperbolicOps.log_map_zero(ent[trip[:, 2]], c))
+        s_tan = self.dropout(HyperbolicOps.log_map_zero(_take(self, ent, trip[:, 0]), c))
+        o_tan = self.dropout(HyperbolicOps.log_map_zero(_take(self, ent, trip[:, 2]), c))
         return HyperbolicOps.exp_map_zero((torch.mm(s_tan, self.W_s) + torch.mm(o_tan, self.W_o)).contiguous(), c)
 
 
@@ -506,8 +516,8 @@ class HyperbolicRotHRel(_RelDecoderBase):
     def _query(self, ent, trip):
         """hyperbolic_decoder.py:1223-1234."""
         c = self.c
-        o_emb = ent[trip[:, 2]].contiguous()
-        s_tan = self.dropout(HyperbolicOps.log_map_zero(ent[trip[:, 0]], c))
+        o_emb = _take(self, ent, trip[:, 2]).contiguous()
+        s_tan = self.dropout(HyperbolicOps.log_map_zero(_take(self, ent, trip[:, 0]), c))
         s_tan = s_tan + _ag.linear(self.reshape_fc2, F.relu(_ag.linear(self.reshape_fc1, s_tan)))
         rot_s = HyperbolicOps.exp_map_zero(givens_rotation(s_tan, self.global_rot).contiguous(), c)
         return HyperbolicOps.mobius_add(-rot_s, o_emb, c)
@@ -540,8 +550,8 @@ class HyperbolicAttHRel(_RelDecoderBase):
     def _query(self, ent, trip):
         """hyperbolic_decoder.py:1605-1628."""
         c = self.c
-        o_emb = ent[trip[:, 2]].contiguous()
-        s_tan = self.dropout(HyperbolicOps.log_map_zero(ent[trip[:, 0]], c))
+        o_emb = _take(self, ent, trip[:, 2]).contiguous()
+        s_tan = self.dropout(HyperbolicOps.log_map_zero(_take(self, ent, trip[:, 0]), c))
         o_tan = HyperbolicOps.log_map_zero(o_emb, c)
         a = torch.sigmoid(torch.mv(torch.cat([s_tan, o_tan], dim=-1), self.attn_weight)).unsqueeze(1)
         mixed = a * givens_rotation(s_tan, self.global_rot) + (1.0 - a) * givens_reflection(s_tan, self.global_ref)
@@ -552,6 +562,8 @@ class HyperbolicAttHRel(_RelDecoderBase):
 class HyperbolicConvTransE(nn.Module):
     """hyperbolic_decoder.py:310-413 (tangent-space ConvTransE; host torch convolution,
     HIP log0; the all-entity product is a plain GEMM)."""
+
+    sorted_lookup = False
 
     def __init__(self, num_entities, embedding_dim, c=0.01, input_dropout=0.0, hidden_dropout=0.0,
                  feature_map_dropout=0.0, channels=50, kernel_size=3):
@@ -571,7 +583,8 @@ class HyperbolicConvTransE(nn.Module):
         et = HyperbolicOps.log_map_zero(entity_embedding.contiguous(), self.c)
         et = 0.9 * torch.tanh(et) + 0.1 * et
         B = len(triplets)
-        x = torch.cat([et[triplets[:, 0]].unsqueeze(1), rel_embedding[triplets[:, 1]].unsqueeze(1)], 1)
+        x = torch.cat([_take(self, et, triplets[:, 0]).unsqueeze(1),
+                       _take(self, rel_embedding, triplets[:, 1]).unsqueeze(1)], 1)
         x = self.feature_map_drop(F.relu(_ag.batch_norm(self.bn1, self.conv1(self.inp_drop(_ag.batch_norm(self.bn0, x))))))
         x = self.hidden_drop(_ag.linear(self.fc, x.view(B, -1)))
         if B > 1:
@@ -581,6 +594,8 @@ class HyperbolicConvTransE(nn.Module):
 
 class HyperbolicConvTransR(nn.Module):
     """hyperbolic_decoder.py:416-510."""
+
+    sorted_lookup = False
 
     def __init__(self, num_relations, embedding_dim, c=0.01, input_dropout=0.0, hidden_dropout=0.0,
                  feature_map_dropout=0.0, channels=50, kernel_size=3):
@@ -600,7 +615,7 @@ class HyperbolicConvTransR(nn.Module):
         et = HyperbolicOps.log_map_zero(entity_embedding.contiguous(), self.c)
         et = 0.9 * torch.tanh(et) + 0.1 * et
         B = len(triplets)
-        x = torch.cat([et[triplets[:, 0]].unsqueeze(1), et[triplets[:, 2]].unsqueeze(1)], 1)
+        x = torch.cat([_take(self, et, triplets[:, 0]).unsqueeze(1), _take(self, et, triplets[:, 2]).unsqueeze(1)], 1)
         x = self.feature_map_drop(F.relu(_ag.batch_norm(self.bn1, self.conv1(self.inp_drop(_ag.batch_norm(self.bn0, x))))))
         x = _ag.batch_norm(self.bn2, self.hidden_drop(_ag.linear(self.fc, x.view(B, -1))))
         return torch.mm(F.relu(x), rel_embedding.transpose(1, 0)) + self.b

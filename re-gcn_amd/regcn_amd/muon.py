@@ -93,3 +93,89 @@ def _run(mats, steps, a, b, c, eps):
         ws = torch.empty(size, device=device, dtype=torch.uint8)
         _lib.launch("regcn_orthogonalize", device, desc, len(live), steps, a, b, c, eps, ws.data_ptr(), size)
     return [o.t() if t else o for o, (_, t) in zip(outs, plans)]
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum with orthogonalised updates for two-dimensional parameters:
+
+        buf = momentum * buf + grad
+        d = grad + momentum * buf          (nesterov; otherwise buf)
+        p = (1 - lr * weight_decay) * p - lr * sqrt(max(1, rows / cols)) * orthogonalize(d)
+
+    One call of `orthogonalize` serves all the parameters of a group (per device).  Parameters without a
+    gradient are left alone; sparse gradients are refused.  The step holds no host synchronisation, so a
+    training step with it can be captured in a HIP graph (training.GraphedSteps)."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS,
+                 eps=1e-7):
+        if not lr >= 0.0:
+            raise ValueError("lr must be >= 0 (got %r)" % (lr,))
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("momentum must be in [0, 1) (got %r)" % (momentum,))
+        if not weight_decay >= 0.0:
+            raise ValueError("weight_decay must be >= 0 (got %r)" % (weight_decay,))
+        if not 1 <= int(steps) <= 1000:
+            raise ValueError("1 to 1000 steps (got %r)" % (steps,))
+        _check_coeffs(*(float(v) for v in coeffs), int(steps))
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, coeffs=tuple(coeffs), eps=eps))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2 or p.dtype not in _lib.DTYPES:
+                self.param_groups.pop()
+                raise ValueError("Muon takes two-dimensional fp32, bf16 or fp16 parameters (got %s %s)"
+                                 % (tuple(p.shape), p.dtype))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_device = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError("Muon does not take sparse gradients")
+                    by_device.setdefault(p.device, []).append(p)
+            for ps in by_device.values():
+                self._update(ps, group)
+        return loss
+
+    def _update(self, ps, group):
+        grads, bufs = [p.grad for p in ps], []
+        for p in ps:
+            st = self.state[p]
+            if "momentum_buffer" not in st:
+                st["momentum_buffer"] = torch.zeros_like(p)
+            bufs.append(st["momentum_buffer"])
+        mu, lr = group["momentum"], group["lr"]
+        torch._foreach_mul_(bufs, mu)
+        torch._foreach_add_(bufs, grads)
+        d = bufs
+        if group["nesterov"]:
+            d = torch._foreach_mul(bufs, mu)
+            torch._foreach_add_(d, grads)
+        o = orthogonalize(d, group["steps"], group["coeffs"], group["eps"])
+        torch._foreach_mul_(o, [max(1.0, p.shape[0] / p.shape[1]) ** 0.5 if p.numel() else 1.0 for p in ps])
+        if group["weight_decay"]:
+            torch._foreach_mul_(ps, 1.0 - lr * group["weight_decay"])
+        torch._foreach_add_(ps, o, alpha=-lr)
+
+
+TABLES = ("dynamic_emb", "emb_rel")  # rows looked up by id: not matrices of a product
+
+
+def split_parameters(model):
+    """(parameters for Muon, the others) of a model: its matrices of at least two rows and columns, but not
+    the entity and relation tables."""
+    mats, rest = [], []
+    for name, p in model.named_parameters():
+        if not p.requires_grad:
+            continue
+        table = name.rsplit(".", 1)[-1] in TABLES
+        (mats if p.dim() == 2 and min(p.shape) > 1 and not table else rest).append(p)
+    return mats, rest

@@ -200,6 +200,25 @@ def construct_snap_r(test_triples, num_nodes, num_rels, final_score, topK):
     return np.array(out, dtype=int).reshape(-1, 3)
 
 
+def construct_snap_sampled(test_triples, num_nodes, num_rels, final_score, draws, u=None, relation=False, **limits):
+    """`construct_snap` (relation: `construct_snap_r`) with drawn answers in place of the top k: the
+    distinct ids of `draws` draws a query (`sample` with its limits, at the numbers u, B x draws, or fresh
+    uniform ones) as next-history triples, in increasing id.  A query without an answer adds none."""
+    B = final_score.shape[0]
+    if u is None:
+        u = torch.rand(B, draws, device=final_score.device, dtype=torch.float64)
+    ids = sample(final_score, u.reshape(B, draws), **limits).cpu().numpy()
+    tri = test_triples.cpu().numpy()
+    out = []
+    for (h, r, t), drawn in zip(tri.tolist(), ids):
+        for x in np.unique(drawn[drawn >= 0]).tolist():
+            if relation:
+                out.append([h, x, t] if x < num_rels else [t, x - num_rels, h])
+            else:
+                out.append([h, r, x] if r < num_rels else [x, r - num_rels, h])
+    return np.array(out, dtype=int).reshape(-1, 3)
+
+
 def load_all_answers_for_filter(total_data, num_rel, rel_p=False):
     """rgcn/utils.py:264-283: {s: {r: {o}}, o: {r + R: {s}}} (or {s: {o: {r}}} for
     relation prediction) over one snapshot's triples."""

@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from torch.nn.parameter import Parameter
 
 from . import autograd as _ag
+from .hyperbolic_decoder import _take
 from .hyperbolic_model import relation_gru_step
 from .layers import UnionRGCNLayer
 
@@ -57,6 +58,8 @@ class RGCNCell(BaseRGCN):
 class ConvTransE(nn.Module):
     """src/decoder.py:55-100."""
 
+    sorted_lookup = False
+
     def __init__(self, num_entities, embedding_dim, input_dropout=0, hidden_dropout=0, feature_map_dropout=0,
                  channels=50, kernel_size=3, use_bias=True):
         super().__init__()
@@ -77,7 +80,8 @@ class ConvTransE(nn.Module):
                 partial_embeding=None):
         e_all = torch.tanh(embedding)
         B = len(triplets)
-        x = torch.cat([e_all[triplets[:, 0]].unsqueeze(1), emb_rel[triplets[:, 1]].unsqueeze(1)], 1)
+        x = torch.cat([_take(self, e_all, triplets[:, 0]).unsqueeze(1),
+                       _take(self, emb_rel, triplets[:, 1]).unsqueeze(1)], 1)
         x = self.feature_map_drop(F.relu(_ag.batch_norm(self.bn1, self.conv1(self.inp_drop(_ag.batch_norm(self.bn0, x))))))
         x = self.hidden_drop(_ag.linear(self.fc, x.view(B, -1)))
         if B > 1:
@@ -88,6 +92,8 @@ class ConvTransE(nn.Module):
 
 class ConvTransR(nn.Module):
     """src/decoder.py:10-52."""
+
+    sorted_lookup = False
 
     def __init__(self, num_relations, embedding_dim, input_dropout=0, hidden_dropout=0, feature_map_dropout=0,
                  channels=50, kernel_size=3, use_bias=True):
@@ -108,7 +114,7 @@ class ConvTransR(nn.Module):
     def forward(self, embedding, emb_rel, triplets, nodes_id=None, mode="train", negative_rate=0):
         e_all = torch.tanh(embedding)
         B = len(triplets)
-        x = torch.cat([e_all[triplets[:, 0]].unsqueeze(1), e_all[triplets[:, 2]].unsqueeze(1)], 1)
+        x = torch.cat([_take(self, e_all, triplets[:, 0]).unsqueeze(1), _take(self, e_all, triplets[:, 2]).unsqueeze(1)], 1)
         x = self.feature_map_drop(F.relu(_ag.batch_norm(self.bn1, self.conv1(self.inp_drop(_ag.batch_norm(self.bn0, x))))))
         x = _ag.batch_norm(self.bn2, self.hidden_drop(_ag.linear(self.fc, x.view(B, -1))))
         return torch.mm(F.relu(x), emb_rel.transpose(1, 0))

@@ -251,6 +251,16 @@ def euclid_model_forward(model, g_list):
     return history, None, h0, [], []
 
 
+def use_sorted_lookup(model, on=True):
+    """The decoders of `model` look entity and relation rows up through autograd.embedding (on) or by torch
+    indexing (off, the default): the same rows and, up to the order of fp32 sums, the same gradients.  Returns
+    the model."""
+    for m in model.modules():
+        if hasattr(type(m), "sorted_lookup"):
+            m.sorted_lookup = bool(on)
+    return model
+
+
 class GraphedSteps:
     """Whole training steps replayed from HIP graphs: one graph per key
     (a training sample: its snapshot shapes fix every launch), captured right after the

@@ -58,3 +58,16 @@ def test_workspace_is_that_of_the_largest_set():
     one = size([(200, 200)])
     assert size([(200, 200)] * 32) == 32 * one == size([(200, 200)] * 70)
     assert size([(200, 200), (4096, 4096)]) == size([(4096, 4096)])  # the tile sizes are sets of their own
+
+
+@pytest.mark.parametrize("kw", [dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1), dict(steps=0),
+                                dict(coeffs=(4.0, 0.0, 0.0))])
+def test_muon_refuses_settings(kw):
+    with pytest.raises(ValueError):
+        muon.Muon([torch.zeros(2, 2, requires_grad=True)], **kw)
+
+
+@pytest.mark.parametrize("p", [torch.zeros(3), torch.zeros(2, 2, 2), torch.zeros(2, 2, dtype=torch.float64)])
+def test_muon_refuses_parameters(p):
+    with pytest.raises(ValueError):
+        muon.Muon([p.requires_grad_(True)])
