@@ -440,6 +440,29 @@ def hyp_ce_loss(q, cand, target, c, bias=None, scale=None, margin=None, reductio
     return loss
 
 
+def _total(x):
+    """x.sum() in stages of 64 elements each.  torch's sum of many elements to one runs over several workgroups
+    and clears its tickets with a memset; in a replayed HIP graph such a sum returned wrong values from
+    the second replay on (the scale's and margin's gradients below).  Sums of 64 stay in one workgroup."""
+    x = x.reshape(-1)
+    while x.numel() > 64:
+        x = torch.nn.functional.pad(x, (0, -x.numel() % 64)).view(-1, 64).sum(1)
+    return x.sum()
+
+
+class _SpreadScalar(torch.autograd.Function):
+    """A 0-dim or one-element tensor over a shape; its gradient is the _total of the shape's."""
+
+    @staticmethod
+    def forward(ctx, s, shape):
+        ctx.shape = s.shape
+        return s.detach().reshape(()).expand(shape).clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return _total(g).reshape(ctx.shape), None
+
+
 def hyp_dist_ce_loss(q, cand, target, c_r, bias=None, scale=None, margin=None, reduction="mean"):
     """mean CE of the arctanh-distance score with per-query curvatures c_r
     (hyperbolic_decoder.py:257-283): logits = scale (margin - d_{c_r}(q, e)) + bias,
@@ -458,9 +481,12 @@ def hyp_dist_ce_loss(q, cand, target, c_r, bias=None, scale=None, margin=None, r
     n = (num2.clamp(min=1e-30).sqrt() / (den + EPS).abs()).clamp(min=EPS)
     n = torch.min(n, 1.0 / (sqrt_c + EPS) - EPS)
     dist = (2.0 / (sqrt_c + EPS)) * torch.atanh((sqrt_c * n).clamp(max=1.0 - EPS))
-    logits = margin.double() - dist if torch.is_tensor(margin) else (0.0 if margin is None else margin) - dist
+    if torch.is_tensor(margin):
+        logits = _SpreadScalar.apply(margin.double(), dist.shape) - dist
+    else:
+        logits = (0.0 if margin is None else margin) - dist
     if scale is not None:
-        logits = scale.double() * logits
+        logits = (_SpreadScalar.apply(scale.double(), dist.shape) if torch.is_tensor(scale) else scale) * logits
     if bias is not None:
         logits = logits + bias.double()
     return torch.nn.functional.cross_entropy(logits, target.long(), reduction=reduction).float()

@@ -68,7 +68,7 @@ def check(score, u, T=1.0, k=0, p=1.0, m=0.0, **kw):
         np.testing.assert_array_equal(g[r], ids, err_msg="row %d" % r)
         fin = np.isfinite(lp)
         np.testing.assert_array_equal(fin, np.isfinite(lg[r]))
-        assert (np.abs(lg[r] - lp)[fin] <= 2.0 ** -24 * np.abs(lp[fin]) * 1.01 + 2.0 ** -22).all()
+        assert (np.abs(lg[r][fin] - lp[fin]) <= 2.0 ** -24 * np.abs(lp[fin]) * 1.01 + 2.0 ** -22).all()
     again = ranking.sample(score, u, temperature=T, top_k=k, top_p=p, min_p=m)
     assert torch.equal(again, got)
 
