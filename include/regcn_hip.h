@@ -866,7 +866,7 @@ typedef struct regcn_matrix {
 /* Newton-Schulz iteration of each matrix on its shorter side: X = G / (|G|_F + eps), then `steps` times
  * A = X X^T, X = a X + (b A + c A A) X, as exact as fp32 products, one rounding to the result's type.
  * a, b, c must keep the iteration of a singular value, s <- a s + b s^3 + c s^5 from [0, 1], within
- * [-4, 4]: the operands are held in fp16 halves.  `mats` is host memory and read before the call returns. */
+ * |s| <= 2 and |b s^2 + c s^4| <= 16: the operands are held in fp16 halves.  `mats` is host memory and read before the call returns. */
 int64_t regcn_orthogonalize_workspace_bytes(const regcn_matrix* mats, int32_t n_mats);
 int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps, float a, float b, float c, float eps,
                         void* workspace, size_t ws_bytes, void* stream);

@@ -7,12 +7,13 @@
 // A A = A (A)^T since A is symmetric, and B X = B (X^T)^T with X^T kept beside X.
 //
 // Precision.  The products' errors are amplified by a^steps along small singular directions, so they
-// are made as exact as fp32 products, on the fp16 matrix cores: an fp32 number x is held as two fp16
-// numbers, x = hi + lo / 2048 with hi = fp16(x) and lo = fp16(2048 (x - hi)) (22 bits and a sign, to
-// 2^-36 in absolute terms), and
-//   P Q^T = hi hi^T + (hi lo^T + lo hi^T) / 2048      (lo lo^T is below 2^-24 of the product)
-// in two fp32 accumulators.  Three fp16 products at 8 times the fp32 matrix rate.  X, A and B stay within
-// fp16's range (|X| <= 1 at the start; the binding refuses coefficients whose iteration leaves [-4, 4]).
+// are made as exact as fp32 products, on the fp16 matrix cores: an fp32 number is held as two fp16
+// numbers, x 2^E = hi + lo, hi and lo the roundings of x 2^E and of what is left (22 bits and a sign; 2^-37
+// in absolute terms for X), and
+//   P Q^T = hi hi^T + hi lo^T + lo hi^T      (lo lo^T is below 2^-24 of the product)
+// in one fp32 accumulator: three fp16 products at 8 times the fp32 matrix rate.  The matrix cores take
+// subnormal halves as they are.  E is 12 for X and A and 11 for B: the binding refuses coefficients whose
+// iteration leaves |s| <= 2 or |b s^2 + c s^4| <= 16, so nothing passes 2^15.
 //
 // Layout of an operand: rows of 8-element groups, each group 8 hi then 8 lo halves: a tile's k-step of
 // 32 is one 128-byte line of a row.  Rows and columns are padded to the tile with zeros, which
@@ -27,10 +28,10 @@ namespace regcn {
 namespace {
 
 constexpr int MAXM = 32;      // matrices in a set of launches
-constexpr int THR = 256;      // four waves, 2 x 2 over the tile
+constexpr int THR = 256;
 constexpr int KSTEP = 32;     // k of a stage: a 128-byte line of each row
 constexpr int NORM_WGS = 1024;  // most partial sums of a norm
-constexpr float LO = 2048.f;  // scale of the low halves
+constexpr float EX = 4096.f, EB = 2048.f;  // 2^E of X and A, of B
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -42,7 +43,9 @@ struct Mat {
   int32_t m, n;     // m <= n
   int32_t trans;    // G holds X^T
   int32_t dtype;
-  int32_t splits;   // of k in A = X X^T
+  struct Cut {
+    int32_t full, splits;  // whole tiles, pieces of k of the others
+  } gram, poly;
 };
 
 struct Job {
@@ -62,7 +65,7 @@ struct Parts {
   __host__ __device__ Parts(const Mat& q) {
     mp = pad_to(q.m, T);
     np = pad_to(q.n, T);
-    const int64_t xb = (int64_t)mp * np * 4, ab = (int64_t)mp * mp * 4, nt = mp / T;
+    const int64_t xb = (int64_t)mp * np * 4, ab = (int64_t)mp * mp * 4;
     xt[0] = 0;
     xt[1] = xb;
     x = 2 * xb;
@@ -70,7 +73,9 @@ struct Parts {
     B = A + ab;
     norm = B + ab;
     split = norm + NORM_WGS * 8;
-    bytes = split + (q.splits > 1 ? q.splits * (nt * (nt + 1) / 2) * T * T * 4 : 0);
+    const int64_t st = T < 128 ? T : 128, nt = mp / st, tri = nt * (nt + 1) / 2;  // the symmetric products' tiles
+    const auto cut = [&](const Mat::Cut& c) { return c.splits > 1 ? (tri - c.full) * c.splits * st * st * 4 : 0; };
+    bytes = split + (cut(q.gram) > cut(q.poly) ? cut(q.gram) : cut(q.poly));
   }
 };
 
@@ -133,7 +138,7 @@ __device__ __forceinline__ void store_group(char* p, const float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     hi[e] = (_Float16)v[e];
-    lo[e] = (_Float16)((v[e] - (float)hi[e]) * LO);
+    lo[e] = (_Float16)(v[e] - (float)hi[e]);
   }
   reinterpret_cast<h8*>(p)[0] = hi;
   reinterpret_cast<h8*>(p)[1] = lo;
@@ -142,7 +147,7 @@ __device__ __forceinline__ void store_group(char* p, const float (&v)[8]) {
 __device__ __forceinline__ void load_group(float (&v)[8], const char* p) {
   const h8 hi = reinterpret_cast<const h8*>(p)[0], lo = reinterpret_cast<const h8*>(p)[1];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e] * (1.f / LO);
+  for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
 }
 
 // X and X^T from G: a 64 x 64 tile of X through LDS.
@@ -172,7 +177,7 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
       v = q.dtype == REGCN_F32    ? ((const float*)q.g)[at]
           : q.dtype == REGCN_BF16 ? (float)((const __bf16*)q.g)[at]
                                   : (float)((const _Float16*)q.g)[at];
-      v /= den;
+      v = v / den * EX;
     }
     tile[q.trans ? lane : r][q.trans ? r : lane] = v;
   }
@@ -197,107 +202,143 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
 // different 16-byte slots of the 64 banks.
 __device__ __forceinline__ int swizzle(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
 
-// C tile (T x T) of P Q^T over `steps` k-steps, added up in fp32 as main + cross / 2048 and left in LDS
-// as [T][T + 1] floats.  p, q: the tile's first rows; ld: bytes of a row.
-template <int T, int STAGES>
+// Shape of a tile: T x T by R x C waves, each FR x FC fragments of 32 x 32.
+template <int T_>
+struct Shape {
+  static constexpr int T = T_;
+  static constexpr int R = 2, C = T == 256 ? 4 : 2, WAVES = R * C, THREADS = 64 * WAVES;
+  static constexpr int FR = T / R / 32, FC = T / C / 32;
+  static constexpr int STAGE = 2 * T * 128, STAGES = T == 64 ? 3 : 2;
+  static constexpr int LOADS = 2 * T / 8 / WAVES;  // 8-row loads of a stage and wave
+  // what is finished at a time: SUB x SUB of the tile, [SUB][SUB + 1] floats in LDS, one per 256 threads
+  static constexpr int SUB = T < 128 ? T : 128, SUBS = THREADS / THR;
+  static constexpr int LDS = STAGES * STAGE > SUBS * SUB * (SUB + 1) * 4 ? STAGES * STAGE : SUBS * SUB * (SUB + 1) * 4;
+};
+
+// P Q^T over `steps` k-steps into this wave's fragments.  p, q: the tile's first rows; ld: bytes of a row.
+// The stages hold 256 rows of T = 128 twice (two workgroups a CU) or 512 rows of T = 256 (one of 8 waves).
+// T = 256 halves what a product reads (L2 to LDS) and, with fragments of 128 x 64 a wave, cuts the LDS reads to
+// three quarters.
+template <typename S>
 __device__ __forceinline__ void product(const char* __restrict__ p, const char* __restrict__ q, int64_t ld, int steps,
-                                        char* lds) {
-  constexpr int W = T / 2, F = W / 32;          // a wave's square of the tile, in 32 x 32 fragments
-  constexpr int LOADS = 2 * T / 8 / 4;          // 8-row loads of a stage and wave
-  constexpr int STAGE = 2 * T * 128;
+                                        char* lds, f16v (&acc)[S::FR][S::FC]) {
+  constexpr int T = S::T;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const char* src[LOADS];
+  const char* src[S::LOADS];
 #pragma unroll
-  for (int u = 0; u < LOADS; ++u) {
-    const int row = (w * LOADS + u) * 8 + (lane >> 3);
+  for (int u = 0; u < S::LOADS; ++u) {
+    const int row = (w * S::LOADS + u) * 8 + (lane >> 3);
     const char* base = row < T ? p + row * ld : q + (int64_t)(row - T) * ld;
     src[u] = base + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
   const auto load = [&](int k, int stage) {
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u)
-      __builtin_amdgcn_global_load_lds((const void*)(src[u] + (int64_t)k * 128),
-                                       (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (w * LOADS + u) * 1024),
-                                       16, 0, 0);
+    for (int u = 0; u < S::LOADS; ++u)
+      __builtin_amdgcn_global_load_lds(
+          (const void*)(src[u] + (int64_t)k * 128),
+          (__attribute__((address_space(3))) void*)(lds + stage * S::STAGE + (w * S::LOADS + u) * 1024), 16, 0, 0);
   };
-  f16v main[F][F] = {}, cross[F][F] = {};
+#pragma unroll
+  for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FC; ++j) acc[i][j] = f16v{};
   const int r32 = lane & 31, half = lane >> 5;
-  const int wr = (w >> 1) * W, wc = T + (w & 1) * W;
-  // stage s is loaded STAGES - 1 steps ahead; one barrier a step: a stage is overwritten only after the
+  const int wr = w / S::C * (T / S::R), wc = T + w % S::C * (T / S::C);
+  // a stage is loaded STAGES - 1 steps ahead; one barrier a step: a stage is overwritten only after the
   // barrier that follows its last reads
-  for (int s = 0; s < STAGES - 1 && s < steps; ++s) load(s, s);
+  for (int s = 0; s < S::STAGES - 1 && s < steps; ++s) load(s, s);
   for (int k = 0; k < steps; ++k) {
-    // this wave's loads of stage k have landed (at most the STAGES - 2 younger stages' are under way)
-    if (STAGES == 3 && k + 1 < steps) {
-      if (LOADS == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
-    if (k + STAGES - 1 < steps) load(k + STAGES - 1, (k + STAGES - 1) % STAGES);
-    const char* st = lds + k % STAGES * STAGE;
+    // this wave's loads of stage k have landed (at most the younger stage's are under way)
+    static_assert(S::STAGES == 2 || S::LOADS == 4, "the wait below counts a stage's loads");
+    if (S::STAGES == 3 && k + 1 < steps) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + S::STAGES - 1 < steps) load(k + S::STAGES - 1, (k + S::STAGES - 1) % S::STAGES);
+    const char* st = lds + k % S::STAGES * S::STAGE;
 #pragma unroll
     for (int kk = 0; kk < KSTEP / 16; ++kk) {
       const int g = 2 * (half + 2 * kk);  // piece of the hi halves of this lane's 8 k
-      h8 ah[F], al[F], bh[F], bl[F];
+      h8 ah[S::FR], al[S::FR], bh[S::FC], bl[S::FC];
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        ah[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g));
-        al[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g + 1));
+      for (int f = 0; f < S::FC; ++f) {
         bh[f] = *reinterpret_cast<const h8*>(st + swizzle(wc + 32 * f + r32, g));
         bl[f] = *reinterpret_cast<const h8*>(st + swizzle(wc + 32 * f + r32, g + 1));
       }
 #pragma unroll
-      for (int i = 0; i < F; ++i)
+      for (int f = 0; f < S::FR; ++f) {
+        ah[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g));
+        al[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g + 1));
+      }
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-          main[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], main[i][j], 0, 0, 0);
-          cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], cross[i][j], 0, 0, 0);
-          cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], cross[i][j], 0, 0, 0);
-        }
+      for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
     }
   }
-  __syncthreads();  // the stages are read: their LDS becomes the tile
-  float* c = (float*)lds;
-#pragma unroll
-  for (int i = 0; i < F; ++i)
-#pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        c[((w >> 1) * W + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3)) * (T + 1) + (w & 1) * W + 32 * j + r32] =
-            main[i][j][r] + cross[i][j][r] * (1.f / LO);
-  __syncthreads();
 }
 
-// The tile in LDS becomes alpha * old + beta * tile (old: the same tile of an operand; null: absent),
-// stored as operand rows at `dst` and, transposed, at `dst_t` (null: not stored), both at the tile's corner.
-template <int T>
+// The tile through LDS in parts: f(c, i, j, thread) for each SUB x SUB part at row i, column j of the tile, its
+// products (times `unscale`) in c, by 256 threads.
+template <typename S, typename F>
+__device__ __forceinline__ void parts_of(const f16v (&acc)[S::FR][S::FC], float unscale, char* lds, F f) {
+  constexpr int SUB = S::SUB, WT = S::T / S::C;  // columns of a wave
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+  constexpr int ROWS = S::T / SUB, COLS = S::T / SUB;  // parts; a row of parts at a time
+  static_assert(S::SUBS == COLS && (ROWS == 1 || S::T / S::R == SUB), "a row of parts is a row of waves, and fits");
+#pragma unroll
+  for (int pr = 0; pr < ROWS; ++pr) {
+    __syncthreads();  // the stages, or the parts before, are read
+    if (ROWS == 1 || w / S::C == pr) {
+      const int row0 = ROWS == 1 ? w / S::C * (S::T / S::R) : 0, col0 = w % S::C * WT;
+      float* c = (float*)lds + col0 / SUB * (SUB * (SUB + 1)) + row0 * (SUB + 1) + col0 % SUB;
+#pragma unroll
+      for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FC; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            c[(32 * i + 8 * (r >> 2) + 4 * half + (r & 3)) * (SUB + 1) + 32 * j + r32] = acc[i][j][r] * unscale;
+    }
+    __syncthreads();
+    const int part = threadIdx.x / THR;
+    f((float*)lds + part * (SUB * (SUB + 1)), pr * SUB, part * SUB, (int)threadIdx.x % THR);
+  }
+}
+
+// The RW x CL part of a tile in LDS becomes alpha * old + beta * part (old: the same of an operand; null: absent),
+// stored as operand rows at `dst` and, transposed, at `dst_t` (null: not stored), both at the part's corner.
+// One barrier of the workgroup.
+template <int RW, int CL>
 __device__ __forceinline__ void finish(float* c, const char* old, float alpha, float beta, char* dst, char* dst_t,
-                                       int64_t ld, int64_t ld_t) {
-  constexpr int G = T / 8;
-  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
+                                       int64_t ld, int64_t ld_t, int thread, int threads) {
+  constexpr int G = CL / 8, LD = CL + 1;
+  for (int it = thread; it < RW * G; it += threads) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
+    if (old) load_group(x, old + r * ld + g * 32);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c[r * (T + 1) + 8 * g + e];
-    if (old) {
-      load_group(x, old + r * ld + g * 32);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = fmaf(alpha, x[e], beta * v[e]);
-        c[r * (T + 1) + 8 * g + e] = v[e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      v[e] = beta * c[r * LD + 8 * g + e];
+      if (old) v[e] = fmaf(alpha, x[e], v[e]);
+      c[r * LD + 8 * g + e] = v[e];
     }
     if (dst) store_group(dst + r * ld + g * 32, v);
   }
-  if (!dst_t) return;
   __syncthreads();
-  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
-    const int col = it / 64 * 16 % T + (it & 15), g = it / 64 * 16 / T * 4 + (it >> 4 & 3);
+  if (!dst_t) return;
+  static_assert(RW % 32 == 0 && CL % 16 == 0, "a wave takes 16 columns of 32 rows");
+  for (int it = thread; it < RW * G; it += threads) {
+    const int col = it / 64 * 16 % CL + (it & 15), g = it / 64 * 16 / CL * 4 + (it >> 4 & 3);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c[(8 * g + e) * (T + 1) + col];
+    for (int e = 0; e < 8; ++e) v[e] = c[(8 * g + e) * LD + col];
     store_group(dst_t + col * ld_t + g * 32, v);
   }
 }
@@ -323,22 +364,23 @@ __device__ __forceinline__ void store_out(const Mat& q, int64_t at, const float 
 
 // The last step's tile into the result, in G's type and orientation.
 template <int T>
-__device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* old, float alpha, int64_t ld, int i0, int j0) {
+__device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* old, float alpha, int64_t ld, int i0, int j0,
+                                           int thread) {
   constexpr int G = T / 8;
-  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
+  for (int it = thread; it < T * G; it += THR) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
     load_group(x, old + r * ld + g * 32);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = fmaf(alpha, x[e], c[r * (T + 1) + 8 * g + e]);
+      v[e] = fmaf(alpha, x[e], c[r * (T + 1) + 8 * g + e]) * (1.f / EX);
       c[r * (T + 1) + 8 * g + e] = v[e];
     }
     if (!q.trans && i0 + r < q.m) store_out(q, (int64_t)(i0 + r) * q.n + j0 + 8 * g, v, q.n - j0 - 8 * g);
   }
-  if (!q.trans) return;
   __syncthreads();
-  for (int it = threadIdx.x; it < T * G; it += blockDim.x) {
+  if (!q.trans) return;
+  for (int it = thread; it < T * G; it += THR) {
     const int col = it / 64 * 16 % T + (it & 15), g = it / 64 * 16 / T * 4 + (it >> 4 & 3);
     float v[8];
 #pragma unroll
@@ -347,108 +389,164 @@ __device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* o
   }
 }
 
-template <int T>
-constexpr int stages() { return T == 64 ? 3 : 2; }
-template <int T>
-constexpr int lds_bytes() {
-  constexpr int a = stages<T>() * 2 * T * 128, b = T * (T + 1) * 4;
-  return a > b ? a : b;
-}
-
-// A = X X^T, upper triangle of tiles, both halves stored; or one of `splits` pieces of k of a tile.
-template <int T>
-__global__ __launch_bounds__(THR, 2) void k_gram(Job job) {
-  __shared__ __align__(16) char lds[lds_bytes<T>()];
-  int wg = blockIdx.x, i, j;
-  const Mat& q = job.mat[find_mat(job, wg)];
-  const Parts<T> w(q);
-  const int nt = w.mp / T, tri = nt * (nt + 1) / 2;
-  const int s = wg / tri, t = wg % tri;
-  triangle(t, nt, i, j);
-  const int64_t ld = (int64_t)w.np * 4;
-  const char* X = q.ws + w.x;
-  const int all = w.np / KSTEP, k0 = (int)((int64_t)all * s / q.splits), k1 = (int)((int64_t)all * (s + 1) / q.splits);
-  product<T, stages<T>()>(X + (int64_t)i * T * ld + k0 * 128, X + (int64_t)j * T * ld + k0 * 128, ld, k1 - k0, lds);
-  float* c = (float*)lds;
-  if (q.splits > 1) {
-    float* part = (float*)(q.ws + w.split) + ((int64_t)s * tri + t) * T * T;
-    for (int it = threadIdx.x; it < T * T; it += THR) part[it] = c[it / T * (T + 1) + it % T];
-    return;
+// Where a workgroup of a symmetric product stands: tile (i, j) of the upper triangle, piece s of k.  The
+// first `full` tiles are whole; the others are cut into `splits` pieces of k each, so that a last round of few
+// tiles (or a matrix of few) still fills the card.
+struct Piece2 {
+  int i, j, t, s;  // t: of the cut tiles, -1: whole
+};
+__device__ __forceinline__ Piece2 symmetric_piece(int wg, int nt, int full, int splits) {
+  Piece2 p{0, 0, -1, 0};
+  const int cut = nt * (nt + 1) / 2 - full;
+  int t = wg;
+  if (wg >= full) {
+    p.t = (wg - full) % cut;
+    p.s = (wg - full) / cut;
+    t = full + p.t;
+    if (splits == 1) p.t = -1;
   }
-  const int64_t la = (int64_t)w.mp * 4;
-  char* A = q.ws + w.A;
-  finish<T>(c, nullptr, 0.f, 1.f, A + i * T * la + j * T * 4, i == j ? nullptr : A + j * T * la + i * T * 4, la, la);
+  triangle(t, nt, p.i, p.j);
+  return p;
 }
 
-// The pieces of k of a tile added up in order: a thread per 4 columns, its pieces' loads under way together.
+// alpha old + beta P P^T of one tile of the upper triangle, both halves stored; or one piece of k of it, stored as
+// fp32 partial sums.
+template <typename S>
+__device__ __forceinline__ void symmetric(const Piece2& at, int splits, const char* P, int64_t ld, int steps, const char* old,
+                                          float alpha, float beta, char* out, int64_t la, float* part, int64_t cut,
+                                          char* lds) {
+  constexpr int T = S::T;
+  static_assert(S::SUB == T, "one part");
+  const int k0 = at.t < 0 ? 0 : (int)((int64_t)steps * at.s / splits);
+  const int k1 = at.t < 0 ? steps : (int)((int64_t)steps * (at.s + 1) / splits);
+  f16v acc[S::FR][S::FC];
+  product<S>(P + (int64_t)at.i * T * ld + k0 * 128, P + (int64_t)at.j * T * ld + k0 * 128, ld, k1 - k0, lds, acc);
+  parts_of<S>(acc, 1.f, lds, [&](float* c, int, int, int thread) {
+    if (at.t >= 0) {
+      float* to = part + (at.s * cut + at.t) * T * T;
+      for (int it = thread; it < T * T; it += THR) to[it] = c[it / T * (T + 1) + it % T];
+      return;
+    }
+    finish<T, T>(c, old ? old + at.i * T * la + at.j * T * 4 : nullptr, alpha, beta, out + at.i * T * la + at.j * T * 4,
+              at.i == at.j ? nullptr : out + at.j * T * la + at.i * T * 4, la, la, thread, THR);
+  });
+}
+
+// The pieces of k of a cut tile added up in order, then as above: a workgroup a strip of 32 rows, a thread per 4
+// columns, its pieces' loads under way together.
+constexpr int STRIP = 32;
 template <int T>
-__global__ __launch_bounds__(T * T / 4 < 1024 ? T * T / 4 : 1024) void k_gram_sum(Job job) {
-  __shared__ __align__(16) float c[T * (T + 1)];
-  int wg = blockIdx.x, i, j;
-  const Mat& q = job.mat[find_mat(job, wg)];
-  const Parts<T> w(q);
-  const int nt = w.mp / T, tri = nt * (nt + 1) / 2;
-  triangle(wg, nt, i, j);
-  const f4* part = (const f4*)(q.ws + w.split) + (int64_t)wg * (T * T / 4);
-  for (int it = threadIdx.x; it < T * T / 4; it += blockDim.x) {
-    f4 v = part[it];
+__device__ __forceinline__ void symmetric_sum(int wg, int nt, int full, int splits, const float* part, const char* old,
+                                              float alpha, float beta, char* out, int64_t la, float* c) {
+  int i, j;
+  const int t = wg / (T / STRIP), r0 = wg % (T / STRIP) * STRIP;
+  triangle(full + t, nt, i, j);
+  const int64_t cut = nt * (nt + 1) / 2 - full;
+  const f4* from = (const f4*)part + (int64_t)t * (T * T / 4) + r0 * (T / 4);
+  for (int it = threadIdx.x; it < STRIP * T / 4; it += THR) {
+    f4 v = from[it];
 #pragma unroll 8
-    for (int s = 1; s < q.splits; ++s) v += part[(int64_t)s * tri * (T * T / 4) + it];
-    const int at = it * 4 / T * (T + 1) + it * 4 % T;
+    for (int s = 1; s < splits; ++s) v += from[s * cut * (T * T / 4) + it];
+    const int to = it * 4 / T * (T + 1) + it * 4 % T;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[at + e] = v[e];
+    for (int e = 0; e < 4; ++e) c[to + e] = v[e];
   }
   __syncthreads();
-  const int64_t la = (int64_t)w.mp * 4;
-  char* A = q.ws + w.A;
-  finish<T>(c, nullptr, 0.f, 1.f, A + i * T * la + j * T * 4, i == j ? nullptr : A + j * T * la + i * T * 4, la, la);
+  const int64_t at = (int64_t)(i * T + r0) * la + j * T * 4;
+  finish<STRIP, T>(c, old ? old + at : nullptr, alpha, beta, out + at,
+                   i == j ? nullptr : out + j * T * la + (i * T + r0) * 4, la, la, threadIdx.x, THR);
 }
 
-// B = b A + c A A, upper triangle of tiles, both halves stored.
-template <int T>
-__global__ __launch_bounds__(THR, 2) void k_poly(Job job) {
-  __shared__ __align__(16) char lds[lds_bytes<T>()];
-  int wg = blockIdx.x, i, j;
+// A = X X^T.  PAD: what the operands are padded to.
+template <int PAD, int T>
+__global__ __launch_bounds__(THR, 2) void k_gram(Job job) {
+  typedef Shape<T> S;
+  __shared__ __align__(16) char lds[S::LDS];
+  int wg = blockIdx.x;
   const Mat& q = job.mat[find_mat(job, wg)];
-  const Parts<T> w(q);
-  triangle(wg, w.mp / T, i, j);
-  const int64_t la = (int64_t)w.mp * 4;
+  const Parts<PAD> w(q);
+  const int nt = w.mp / T;
+  symmetric<S>(symmetric_piece(wg, nt, q.gram.full, q.gram.splits), q.gram.splits, q.ws + w.x, (int64_t)w.np * 4,
+               w.np / KSTEP, nullptr, 0.f, 1.f / EX, q.ws + w.A, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
+               nt * (nt + 1) / 2 - q.gram.full, lds);
+}
+template <int PAD, int T>
+__global__ __launch_bounds__(THR) void k_gram_sum(Job job) {
+  __shared__ __align__(16) float c[STRIP * (T + 1)];
+  int wg = blockIdx.x;
+  const Mat& q = job.mat[find_mat(job, wg)];
+  const Parts<PAD> w(q);
+  symmetric_sum<T>(wg, w.mp / T, q.gram.full, q.gram.splits, (const float*)(q.ws + w.split), nullptr, 0.f, 1.f / EX,
+                   q.ws + w.A, (int64_t)w.mp * 4, c);
+}
+
+// B = b A + c A A.
+template <int PAD, int T>
+__global__ __launch_bounds__(THR, 2) void k_poly(Job job) {
+  typedef Shape<T> S;
+  __shared__ __align__(16) char lds[S::LDS];
+  int wg = blockIdx.x;
+  const Mat& q = job.mat[find_mat(job, wg)];
+  const Parts<PAD> w(q);
+  const int nt = w.mp / T;
   const char* A = q.ws + w.A;
-  char* B = q.ws + w.B;
-  product<T, stages<T>()>(A + i * T * la, A + j * T * la, la, w.mp / KSTEP, lds);
-  finish<T>((float*)lds, A + i * T * la + j * T * 4, job.b, job.c, B + i * T * la + j * T * 4,
-            i == j ? nullptr : B + j * T * la + i * T * 4, la, la);
+  symmetric<S>(symmetric_piece(wg, nt, q.poly.full, q.poly.splits), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
+               job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
+               nt * (nt + 1) / 2 - q.poly.full, lds);
+}
+template <int PAD, int T>
+__global__ __launch_bounds__(THR) void k_poly_sum(Job job) {
+  __shared__ __align__(16) float c[STRIP * (T + 1)];
+  int wg = blockIdx.x;
+  const Mat& q = job.mat[find_mat(job, wg)];
+  const Parts<PAD> w(q);
+  symmetric_sum<T>(wg, w.mp / T, q.poly.full, q.poly.splits, (const float*)(q.ws + w.split), q.ws + w.A,
+                   job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, c);
 }
 
 // X = a X + B X: X in place (a tile is read by its own workgroup only), X^T into its other copy; the last
 // step writes the result instead.
 template <int T>
-__global__ __launch_bounds__(THR, 2) void k_update(Job job) {
-  __shared__ __align__(16) char lds[lds_bytes<T>()];
+__global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
+  typedef Shape<T> S;
+  constexpr int SUB = S::SUB;
+  __shared__ __align__(16) char lds[S::LDS];
   int wg = blockIdx.x;
-  const Mat& q = job.mat[find_mat(job, wg)];
+  const Mat q = job.mat[find_mat(job, wg)];
   const Parts<T> w(q);
-  const int mt = w.mp / T, i = wg % mt, j = wg / mt;
+  const int mt = w.mp / T, i0 = wg % mt * T, j0 = wg / mt * T;
   const int64_t la = (int64_t)w.mp * 4, lx = (int64_t)w.np * 4;
-  product<T, stages<T>()>(q.ws + w.B + i * T * la, q.ws + w.xt[job.side] + j * T * la, la, w.mp / KSTEP, lds);
-  char* X = q.ws + w.x + i * T * lx + (int64_t)j * T * 4;
-  if (job.last)
-    finish_out<T>(q, (float*)lds, X, job.a, lx, i * T, j * T);
-  else
-    finish<T>((float*)lds, X, job.a, 1.f, X, q.ws + w.xt[1 - job.side] + j * T * la + (int64_t)i * T * 4, lx, la);
+  f16v acc[S::FR][S::FC];
+  product<S>(q.ws + w.B + i0 * la, q.ws + w.xt[job.side] + j0 * la, la, w.mp / KSTEP, lds, acc);
+  parts_of<S>(acc, 1.f / EB, lds, [&](float* c, int pi, int pj, int thread) {
+    const int i = i0 + pi, j = j0 + pj;
+    char* X = q.ws + w.x + i * lx + (int64_t)j * 4;
+    if (job.last)
+      finish_out<SUB>(q, c, X, job.a, lx, i, j, thread);
+    else
+      finish<SUB, SUB>(c, X, job.a, 1.f, X, q.ws + w.xt[1 - job.side] + j * la + (int64_t)i * 4, lx, la, thread, THR);
+  });
 }
 
 // ---------------------------------------------------------------------------------------- host
-// Tiles of 128 fill the card from 192 tiles of X on; below that tiles of 64 give four times the workgroups.
-bool wide_tiles(const Mat& q) { return (int64_t)((q.m + 127) / 128) * ((q.n + 127) / 128) >= 192; }
+// The tile of X: 256 from 192 of those on (a workgroup a CU), 128 from 192 of those on; below that tiles of 64
+// give four times the workgroups.  The symmetric products take tiles of at most 128 (256 would leave half of the
+// CUs idle at 4096).
+int tile_of(const Mat& q) {
+  const auto tiles = [&](int t) { return (int64_t)((q.m + t - 1) / t) * ((q.n + t - 1) / t); };
+  return tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+}
 
-int tile_of(const Mat& q) { return wide_tiles(q) ? 128 : 64; }
-
-// Pieces of k in X X^T: enough for about 512 workgroups, each of at least 24 k-steps (about 6 us: the
-// second launch that adds them up costs 4).
-int gram_splits(const Mat& q) {
-  const int t = tile_of(q), nt = (q.m + t - 1) / t, tri = nt * (nt + 1) / 2, steps = pad_to(q.n, t) / KSTEP;
-  return std::max(1, std::min({512 / tri, steps / 24, 32}));
+// Which tiles of a symmetric product over `steps` k-steps are cut along k.  Fewer than half of what the card
+// holds (two workgroups a CU): cut into pieces of at least 24 k-steps (about 6 us; the second launch that adds them
+// up costs 4).  More: a last round that fills less than half of it is cut (4096: 16 of 528 tiles; 280 -> 220 us).
+Mat::Cut cut_of(int tri, int steps) {
+  const int slots = 512, rest = tri % slots;
+  const int full = tri - rest;
+  if (rest == 0 || rest > slots / 2) return {tri, 1};
+  const int splits = full ? std::min({slots / rest, steps / 8, 8}) : std::min({slots / rest, steps / 24, 32});
+  if (splits < 2) return {tri, 1};
+  return {full, splits};
 }
 
 template <typename F>
@@ -460,28 +558,34 @@ int layout(Job& job, F wgs_of) {
 
 template <int T>
 int run_set(Job& job, int steps, hipStream_t st) {
+  constexpr int ST = T < 128 ? T : 128;
   int n = layout(job, [](const Mat& q) { return norm_parts((int64_t)q.m * q.n); });
   k_norm<T><<<n, THR, 0, st>>>(job);
   n = layout(job, [](const Mat& q) { return pad_to(q.m, T) / 64 * (pad_to(q.n, T) / 64); });
   k_split<T><<<n, THR, 0, st>>>(job);
-  const auto tri = [](const Mat& q) { const int nt = pad_to(q.m, T) / T; return nt * (nt + 1) / 2; };
+  const auto tri = [](const Mat& q) { const int nt = pad_to(q.m, T) / ST; return nt * (nt + 1) / 2; };
+  const auto wgs = [&](const Mat& q, const Mat::Cut& c) { return c.full + (tri(q) - c.full) * c.splits; };
+  const auto sums = [&](const Mat& q, const Mat::Cut& c) { return c.splits > 1 ? (tri(q) - c.full) * (ST / STRIP) : 0; };
   for (int s = 0; s < steps; ++s) {
-    n = layout(job, [&](const Mat& q) { return tri(q) * q.splits; });
-    k_gram<T><<<n, THR, 0, st>>>(job);
-    n = layout(job, [&](const Mat& q) { return q.splits > 1 ? tri(q) : 0; });
-    if (n) k_gram_sum<T><<<n, std::min(1024, T * T / 4), 0, st>>>(job);
-    n = layout(job, tri);
-    k_poly<T><<<n, THR, 0, st>>>(job);
+    n = layout(job, [&](const Mat& q) { return wgs(q, q.gram); });
+    k_gram<T, ST><<<n, THR, 0, st>>>(job);
+    n = layout(job, [&](const Mat& q) { return sums(q, q.gram); });
+    if (n) k_gram_sum<T, ST><<<n, THR, 0, st>>>(job);
+    n = layout(job, [&](const Mat& q) { return wgs(q, q.poly); });
+    k_poly<T, ST><<<n, THR, 0, st>>>(job);
+    n = layout(job, [&](const Mat& q) { return sums(q, q.poly); });
+    if (n) k_poly_sum<T, ST><<<n, THR, 0, st>>>(job);
     n = layout(job, [](const Mat& q) { return pad_to(q.m, T) / T * (pad_to(q.n, T) / T); });
     job.side = s & 1;
     job.last = s == steps - 1;
-    k_update<T><<<n, THR, 0, st>>>(job);
+    k_update<T><<<n, Shape<T>::THREADS, 0, st>>>(job);
   }
   return check_launch("orthogonalize");
 }
 
 int64_t mat_bytes(const Mat& q) {
-  const int64_t b = wide_tiles(q) ? Parts<128>(q).bytes : Parts<64>(q).bytes;
+  const int t = tile_of(q);
+  const int64_t b = t == 256 ? Parts<256>(q).bytes : t == 128 ? Parts<128>(q).bytes : Parts<64>(q).bytes;
   return (b + 255) / 256 * 256;
 }
 
@@ -498,21 +602,23 @@ int to_mat(const regcn_matrix& d, Mat& q) {
   q.n = (int)std::max(d.rows, d.cols);
   q.dtype = d.dtype;
   if ((int64_t)q.m * q.n > (1ll << 40)) return set_error(REGCN_ENOTSUP, "orthogonalize: up to 2^40 elements");
-  q.splits = gram_splits(q);
+  const int t = tile_of(q), st = std::min(t, 128), nt = pad_to(q.m, t) / st, tri = nt * (nt + 1) / 2;
+  q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP);
+  q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP);
   return 0;
 }
 
 // Matrices in sets: one tile size, at most MAXM.
 template <typename F>
 int for_sets(const regcn_matrix* mats, int count, F run) {
-  for (int wide = 0; wide < 2; ++wide) {
+  for (int tile = 64; tile <= 256; tile *= 2) {
     Job job{};
     for (int k = 0; k < count; ++k) {
       Mat q;
       if (int rc = to_mat(mats[k], q)) return rc;
-      if (wide_tiles(q) == (bool)wide) job.mat[job.count++] = q;
+      if (tile_of(q) == tile) job.mat[job.count++] = q;
       if (job.count == MAXM || (k == count - 1 && job.count)) {
-        if (int rc = run(job, wide)) return rc;
+        if (int rc = run(job, tile)) return rc;
         job = Job{};
       }
     }
@@ -548,7 +654,7 @@ int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float
   const int64_t need = orthogonalize_ws_bytes(mats, count);
   if (!ws || (int64_t)ws_bytes < need)
     return set_error(REGCN_EINVAL, "orthogonalize: workspace of %zu bytes, needs %lld", ws_bytes, (long long)need);
-  return for_sets(mats, count, [&](Job& job, int wide) {
+  return for_sets(mats, count, [&](Job& job, int tile) {
     char* p = (char*)ws;
     for (int q = 0; q < job.count; ++q) {
       job.mat[q].ws = p;
@@ -558,7 +664,9 @@ int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float
     job.b = b;
     job.c = c;
     job.eps = eps;
-    return wide ? run_set<128>(job, steps, st) : run_set<64>(job, steps, st);
+    return tile == 256   ? run_set<256>(job, steps, st)
+           : tile == 128 ? run_set<128>(job, steps, st)
+                         : run_set<64>(job, steps, st);
   });
 }
 

@@ -15,7 +15,7 @@ import torch
 from . import _lib
 
 COEFFS = (3.4445, -4.7750, 2.0315)
-_LIMIT = 4.0
+_LIMIT, _LIMIT_B = 2.0, 16.0
 
 
 @functools.lru_cache(maxsize=64)
@@ -24,9 +24,11 @@ def _check_coeffs(a, b, c, steps):
     small.  A grid of 2049 starts, finer than the polynomial turns."""
     s = torch.linspace(0, 1, 2049, dtype=torch.float64)
     for _ in range(steps):
-        s = a * s + b * s ** 3 + c * s ** 5
-        if not bool((s.abs() <= _LIMIT).all()):  # NaN and infinities too
-            raise ValueError("coefficients %r leave [-%g, %g] within %d steps" % ((a, b, c), _LIMIT, _LIMIT, steps))
+        poly = b * s ** 2 + c * s ** 4
+        s = a * s + s * poly
+        if not bool((s.abs() <= _LIMIT).all() and (poly.abs() <= _LIMIT_B).all()):  # NaN and infinities too
+            raise ValueError("coefficients %r leave |s| <= %g or |b s^2 + c s^4| <= %g within %d steps"
+                             % ((a, b, c), _LIMIT, _LIMIT_B, steps))
 
 
 def _plan(g):

@@ -89,9 +89,9 @@ def test_sizes(m, n, kind, dt):
     assert torch.equal(out, muon.orthogonalize(G))  # the same bits on every call
 
 
-@pytest.mark.parametrize("m,n", [(1700, 1701), (1921, 1600), (129, 30011)])
+@pytest.mark.parametrize("m,n", [(1700, 1701), (1921, 1600), (129, 30011), (3585, 3500), (500, 28001)])
 def test_wide_tiles(m, n):
-    """From 192 tiles of 128 on: ragged sides, both orientations, k in pieces."""
+    """From 192 tiles of 128, and of 256, on: ragged sides, both orientations, k in pieces, a cut last round."""
     for kind in ("flat", "decay"):
         G = matrix(m, n, 3, F32, kind)
         check(muon.orthogonalize(G), G)

@@ -13,7 +13,7 @@ G = torch.zeros(4, 8)
     (G, {}, ValueError), (G.double(), {}, TypeError), (G[0], {}, ValueError), (G.numpy(), {}, TypeError),
     ([G, None], {}, TypeError), (G, dict(steps=0), ValueError), (G, dict(steps=2000), ValueError),
     (G, dict(coeffs=(3.0, 0.0, 0.0)), ValueError), (G, dict(coeffs=(1.0, 2.0)), ValueError),
-    (G, dict(coeffs=(float("nan"), 0.0, 0.0)), ValueError), (G, dict(eps=-1.0), ValueError),
+    (G, dict(coeffs=(float("nan"), 0.0, 0.0)), ValueError), (G, dict(coeffs=(20.0, -40.0, 20.0)), ValueError), (G, dict(eps=-1.0), ValueError),
     (G, dict(eps=float("inf")), ValueError), ([G.view(2, 2, 8)], {}, ValueError)])
 def test_orthogonalize_refuses(g, kw, err):
     with pytest.raises(err):
