@@ -215,72 +215,100 @@ struct Shape {
   static constexpr int LDS = STAGES * STAGE > SUBS * SUB * (SUB + 1) * 4 ? STAGES * STAGE : SUBS * SUB * (SUB + 1) * 4;
 };
 
+// 16 bytes a lane from base + voff + soff to LDS, lane l's at dst + 16 l.
+__device__ __forceinline__ void load_lds(char* base, int voff, int soff, char* dst) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, (short)0, -1, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, voff, soff, 0, 0);
+}
+
 // P Q^T over `steps` k-steps into this wave's fragments.  p, q: the tile's first rows; ld: bytes of a row.
 // The stages hold 256 rows of T = 128 twice (two workgroups a CU) or 512 rows of T = 256 (one of 8 waves).
 // T = 256 halves what a product reads (L2 to LDS) and, with fragments of 128 x 64 a wave, cuts the LDS reads to
 // three quarters.
+//
+// Two half steps of 16 k alternate, each with fragments of its own: while the matrix cores work on one half's,
+// the other's are read, and in the second half the next stage's first.  The barrier stands between
+// the halves: behind it every wave has read all of stage k, whose place the loads of stage k + STAGES take, and
+// stage k + 1 has landed.  So neither an LDS read nor a load is waited for right after its issue.
 template <typename S>
 __device__ __forceinline__ void product(const char* __restrict__ p, const char* __restrict__ q, int64_t ld, int steps,
                                         char* lds, f16v (&acc)[S::FR][S::FC]) {
   constexpr int T = S::T;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const char* src[S::LOADS];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the first half of the waves loads P's rows, the other Q's: 32-bit offsets from a buffer resource
+  const bool of_p = w < S::WAVES / 2;
+  char* const base = const_cast<char*>(of_p ? p : q);
+  int voff[S::LOADS];
 #pragma unroll
   for (int u = 0; u < S::LOADS; ++u) {
-    const int row = (w * S::LOADS + u) * 8 + (lane >> 3);
-    const char* base = row < T ? p + row * ld : q + (int64_t)(row - T) * ld;
-    src[u] = base + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    const int row = (w % (S::WAVES / 2) * S::LOADS + u) * 8 + (lane >> 3);
+    voff[u] = (int)(row * ld) + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
   }
   const auto load = [&](int k, int stage) {
 #pragma unroll
-    for (int u = 0; u < S::LOADS; ++u)
-      __builtin_amdgcn_global_load_lds(
-          (const void*)(src[u] + (int64_t)k * 128),
-          (__attribute__((address_space(3))) void*)(lds + stage * S::STAGE + (w * S::LOADS + u) * 1024), 16, 0, 0);
+    for (int u = 0; u < S::LOADS; ++u) load_lds(base, voff[u], k * 128, lds + stage * S::STAGE + (w * S::LOADS + u) * 1024);
   };
 #pragma unroll
   for (int i = 0; i < S::FR; ++i)
 #pragma unroll
     for (int j = 0; j < S::FC; ++j) acc[i][j] = f16v{};
   const int r32 = lane & 31, half = lane >> 5;
-  const int wr = w / S::C * (T / S::R), wc = T + w % S::C * (T / S::C);
-  // a stage is loaded STAGES - 1 steps ahead; one barrier a step: a stage is overwritten only after the
-  // barrier that follows its last reads
-  for (int s = 0; s < S::STAGES - 1 && s < steps; ++s) load(s, s);
-  for (int k = 0; k < steps; ++k) {
-    // this wave's loads of stage k have landed (at most the younger stage's are under way)
-    static_assert(S::STAGES == 2 || S::LOADS == 4, "the wait below counts a stage's loads");
-    if (S::STAGES == 3 && k + 1 < steps) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  const int wr = w / S::C * (T / S::R) + r32, wc = T + w % S::C * (T / S::C) + r32;
+  struct Half {
+    h8 ah[S::FR], al[S::FR], bh[S::FC], bl[S::FC];
+  };
+  const auto read = [&](Half& f, const char* st, int kk) {
+    const int g = 2 * (half + 2 * kk);  // piece of the hi halves of this lane's 8 k
+#pragma unroll
+    for (int i = 0; i < S::FC; ++i) f.bh[i] = *reinterpret_cast<const h8*>(st + swizzle(wc, g) + i * 4096);
+#pragma unroll
+    for (int i = 0; i < S::FR; ++i) f.ah[i] = *reinterpret_cast<const h8*>(st + swizzle(wr, g) + i * 4096);
+#pragma unroll
+    for (int i = 0; i < S::FC; ++i) f.bl[i] = *reinterpret_cast<const h8*>(st + swizzle(wc, g + 1) + i * 4096);
+#pragma unroll
+    for (int i = 0; i < S::FR; ++i) f.al[i] = *reinterpret_cast<const h8*>(st + swizzle(wr, g + 1) + i * 4096);
+  };
+  const auto multiply = [&](const Half& f) {
+#pragma unroll
+    for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FC; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FC; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < S::FR; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FC; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
+  };
+  // all but the loads of the STAGES - 2 younger stages have landed, for every wave
+  static_assert(S::STAGES == 2 || (S::STAGES == 3 && S::LOADS == 4), "the wait counts a stage's loads");
+  const auto wait = [&](bool younger) {
+    if (S::STAGES == 3 && younger) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k + S::STAGES - 1 < steps) load(k + S::STAGES - 1, (k + S::STAGES - 1) % S::STAGES);
-    const char* st = lds + k % S::STAGES * S::STAGE;
-#pragma unroll
-    for (int kk = 0; kk < KSTEP / 16; ++kk) {
-      const int g = 2 * (half + 2 * kk);  // piece of the hi halves of this lane's 8 k
-      h8 ah[S::FR], al[S::FR], bh[S::FC], bl[S::FC];
-#pragma unroll
-      for (int f = 0; f < S::FC; ++f) {
-        bh[f] = *reinterpret_cast<const h8*>(st + swizzle(wc + 32 * f + r32, g));
-        bl[f] = *reinterpret_cast<const h8*>(st + swizzle(wc + 32 * f + r32, g + 1));
-      }
-#pragma unroll
-      for (int f = 0; f < S::FR; ++f) {
-        ah[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g));
-        al[f] = *reinterpret_cast<const h8*>(st + swizzle(wr + 32 * f + r32, g + 1));
-      }
-#pragma unroll
-      for (int i = 0; i < S::FR; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < S::FR; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < S::FR; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+  };
+  for (int s = 0; s < S::STAGES - 1 && s < steps; ++s) load(s, s);
+  wait(S::STAGES == 3 && steps > 1);
+  if (S::STAGES - 1 < steps) load(S::STAGES - 1, S::STAGES - 1);
+  Half even, odd;
+  read(even, lds, 0);
+  for (int k = 0; k < steps; ++k) {
+    read(odd, lds + k % S::STAGES * S::STAGE, 1);
+    __builtin_amdgcn_sched_barrier(0);  // the reads go out before the products
+    multiply(even);
+    __builtin_amdgcn_sched_barrier(0);
+    if (k + 1 < steps) {
+      wait(k + 2 < steps);
+      if (k + S::STAGES < steps) load(k + S::STAGES, k % S::STAGES);
+      read(even, lds + (k + 1) % S::STAGES * S::STAGE, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(odd);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -355,17 +383,17 @@ __device__ __forceinline__ void store8(E* p, const float (&v)[8], int m) {
   }
 }
 
-__device__ __forceinline__ void store_out(const Mat& q, int64_t at, const float (&v)[8], int m) {
+__device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, const float (&v)[8], int m) {
   if (m <= 0) return;
-  if (q.dtype == REGCN_F32) store8((float*)q.out + at, v, m);
-  else if (q.dtype == REGCN_BF16) store8((__bf16*)q.out + at, v, m);
-  else store8((_Float16*)q.out + at, v, m);
+  if (dtype == REGCN_F32) store8((float*)out + at, v, m);
+  else if (dtype == REGCN_BF16) store8((__bf16*)out + at, v, m);
+  else store8((_Float16*)out + at, v, m);
 }
 
 // The last step's tile into the result, in G's type and orientation.
 template <int T>
-__device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* old, float alpha, int64_t ld, int i0, int j0,
-                                           int thread) {
+__device__ __forceinline__ void finish_out(void* out, int dtype, bool trans, int m, int n, float* c, const char* old,
+                                           float alpha, int64_t ld, int i0, int j0, int thread) {
   constexpr int G = T / 8;
   for (int it = thread; it < T * G; it += THR) {
     const int r = it / G, g = it % G;
@@ -376,16 +404,16 @@ __device__ __forceinline__ void finish_out(const Mat& q, float* c, const char* o
       v[e] = fmaf(alpha, x[e], c[r * (T + 1) + 8 * g + e]) * (1.f / EX);
       c[r * (T + 1) + 8 * g + e] = v[e];
     }
-    if (!q.trans && i0 + r < q.m) store_out(q, (int64_t)(i0 + r) * q.n + j0 + 8 * g, v, q.n - j0 - 8 * g);
+    if (!trans && i0 + r < m) store_out(out, dtype, (int64_t)(i0 + r) * n + j0 + 8 * g, v, n - j0 - 8 * g);
   }
   __syncthreads();
-  if (!q.trans) return;
+  if (!trans) return;
   for (int it = thread; it < T * G; it += THR) {
     const int col = it / 64 * 16 % T + (it & 15), g = it / 64 * 16 / T * 4 + (it >> 4 & 3);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = c[(8 * g + e) * (T + 1) + col];
-    if (j0 + col < q.n) store_out(q, (int64_t)(j0 + col) * q.m + i0 + 8 * g, v, q.m - i0 - 8 * g);
+    if (j0 + col < n) store_out(out, dtype, (int64_t)(j0 + col) * m + i0 + 8 * g, v, m - i0 - 8 * g);
   }
 }
 
@@ -512,19 +540,23 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
   constexpr int SUB = S::SUB;
   __shared__ __align__(16) char lds[S::LDS];
   int wg = blockIdx.x;
-  const Mat q = job.mat[find_mat(job, wg)];
+  const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<T> w(q);
+  char* const ws = q.ws;
+  void* const result = q.out;
+  const int m = q.m, n = q.n, dtype = q.dtype;
+  const bool trans = q.trans;
   const int mt = w.mp / T, i0 = wg % mt * T, j0 = wg / mt * T;
   const int64_t la = (int64_t)w.mp * 4, lx = (int64_t)w.np * 4;
   f16v acc[S::FR][S::FC];
-  product<S>(q.ws + w.B + i0 * la, q.ws + w.xt[job.side] + j0 * la, la, w.mp / KSTEP, lds, acc);
+  product<S>(ws + w.B + i0 * la, ws + w.xt[job.side] + j0 * la, la, w.mp / KSTEP, lds, acc);
   parts_of<S>(acc, 1.f / EB, lds, [&](float* c, int pi, int pj, int thread) {
     const int i = i0 + pi, j = j0 + pj;
-    char* X = q.ws + w.x + i * lx + (int64_t)j * 4;
+    char* X = ws + w.x + i * lx + (int64_t)j * 4;
     if (job.last)
-      finish_out<SUB>(q, c, X, job.a, lx, i, j, thread);
+      finish_out<SUB>(result, dtype, trans, m, n, c, X, job.a, lx, i, j, thread);
     else
-      finish<SUB, SUB>(c, X, job.a, 1.f, X, q.ws + w.xt[1 - job.side] + j * la + (int64_t)i * 4, lx, la, thread, THR);
+      finish<SUB, SUB>(c, X, job.a, 1.f, X, ws + w.xt[1 - job.side] + j * la + (int64_t)i * 4, lx, la, thread, THR);
   });
 }
 
