@@ -237,7 +237,9 @@ __device__ __forceinline__ void product(const char* __restrict__ p, const char* 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // the first half of the waves loads P's rows, the other Q's: 32-bit offsets from a buffer resource
   const bool of_p = w < S::WAVES / 2;
-  char* const base = const_cast<char*>(of_p ? p : q);
+  const uint64_t from = (uint64_t)(of_p ? p : q);  // in scalar registers: a resource in vector ones is looped over
+  char* const base = (char*)((uint64_t)__builtin_amdgcn_readfirstlane((int)(from >> 32)) << 32 |
+                             (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)from));
   int voff[S::LOADS];
 #pragma unroll
   for (int u = 0; u < S::LOADS; ++u) {
@@ -285,31 +287,53 @@ __device__ __forceinline__ void product(const char* __restrict__ p, const char* 
       for (int j = 0; j < S::FC; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
   };
-  // all but the loads of the STAGES - 2 younger stages have landed, for every wave
+  // All but the loads of the STAGES - 2 younger stages have landed, for every wave.  No branch in the loop: past
+  // the last stage it is loaded again, into a place that nobody reads.
   static_assert(S::STAGES == 2 || (S::STAGES == 3 && S::LOADS == 4), "the wait counts a stage's loads");
-  const auto wait = [&](bool younger) {
-    if (S::STAGES == 3 && younger) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  const auto wait = [&] {
+    if (S::STAGES == 3) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  for (int s = 0; s < S::STAGES - 1 && s < steps; ++s) load(s, s);
-  wait(S::STAGES == 3 && steps > 1);
-  if (S::STAGES - 1 < steps) load(S::STAGES - 1, S::STAGES - 1);
+  const int last = steps - 1;
+  for (int s = 0; s < S::STAGES - 1; ++s) load(min(s, last), s);
+  wait();
+  load(min(S::STAGES - 1, last), S::STAGES - 1);
   Half even, odd;
   read(even, lds, 0);
-  for (int k = 0; k < steps; ++k) {
-    read(odd, lds + k % S::STAGES * S::STAGE, 1);
-    __builtin_amdgcn_sched_barrier(0);  // the reads go out before the products
+  // reads, loads and products interleaved one by one, so that the matrix cores never wait for a run of issues
+  constexpr int NM = 3 * S::FR * S::FC, NR = 2 * (S::FR + S::FC), NL = S::LOADS;
+  int at = 0, next = S::STAGE;  // stage k, stage k + 1
+  for (int k = 0; k < last; ++k) {
+    read(odd, lds + at, 1);
     multiply(even);
-    __builtin_amdgcn_sched_barrier(0);
-    if (k + 1 < steps) {
-      wait(k + 2 < steps);
-      if (k + S::STAGES < steps) load(k + S::STAGES, k % S::STAGES);
-      read(even, lds + (k + 1) % S::STAGES * S::STAGE, 0);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x8, NM / NR, 0);  // product
     }
     __builtin_amdgcn_sched_barrier(0);
+    wait();
+    read(even, lds + next, 0);
+    load(min(k + S::STAGES, last), at / S::STAGE);
     multiply(odd);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);  // load
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    }
     __builtin_amdgcn_sched_barrier(0);
+    at = next;
+    next = next == (S::STAGES - 1) * S::STAGE ? 0 : next + S::STAGE;
   }
+  read(odd, lds + at, 1);
+  multiply(even);
+  multiply(odd);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end, before the stages become the tile
 }
 
 // The tile through LDS in parts: f(c, i, j, thread) for each SUB x SUB part at row i, column j of the tile, its
