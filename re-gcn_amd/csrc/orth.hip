@@ -61,13 +61,14 @@ __host__ __device__ inline int pad_to(int v, int t) { return (v + t - 1) / t * t
 template <int T>
 struct Parts {
   int mp, np;
-  int64_t xt[2], x, A, B, norm, split, bytes;
+  int64_t xb, x, A, B, norm, split, bytes;
+  // X^T's two copies (no array: indexed by an argument it would lie in scratch memory)
+  __host__ __device__ int64_t xt(int side) const { return side ? xb : 0; }
   __host__ __device__ Parts(const Mat& q) {
     mp = pad_to(q.m, T);
     np = pad_to(q.n, T);
-    const int64_t xb = (int64_t)mp * np * 4, ab = (int64_t)mp * mp * 4;
-    xt[0] = 0;
-    xt[1] = xb;
+    xb = (int64_t)mp * np * 4;
+    const int64_t ab = (int64_t)mp * mp * 4;
     x = 2 * xb;
     A = 3 * xb;
     B = A + ab;
@@ -170,20 +171,26 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
   const int nt = w.np / 64, i0 = wg / nt * 64, j0 = wg % nt * 64;
   const int rows = q.trans ? q.n : q.m, cols = q.trans ? q.m : q.n;  // as stored
   const int r0 = q.trans ? j0 : i0, c0 = q.trans ? i0 : j0;
-  for (int r = threadIdx.x >> 6; r < 64; r += THR / WAVE) {
-    float v = 0.f;
-    if (r0 + r < rows && c0 + lane < cols) {
-      const int64_t at = (int64_t)(r0 + r) * cols + c0 + lane;
-      v = q.dtype == REGCN_F32    ? ((const float*)q.g)[at]
-          : q.dtype == REGCN_BF16 ? (float)((const __bf16*)q.g)[at]
-                                  : (float)((const _Float16*)q.g)[at];
-      v = v / den * EX;
+  constexpr int PER = 64 / (THR / WAVE);  // this wave's rows, their loads under way together
+  float v[PER];
+  const auto read = [&](const auto* g) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int r = r0 + (threadIdx.x >> 6) + u * (THR / WAVE), c = c0 + lane;
+      v[u] = r < rows && c < cols ? (float)g[(int64_t)r * cols + c] : 0.f;
     }
-    tile[q.trans ? lane : r][q.trans ? r : lane] = v;
+  };
+  if (q.dtype == REGCN_F32) read((const float*)q.g);
+  else if (q.dtype == REGCN_BF16) read((const __bf16*)q.g);
+  else read((const _Float16*)q.g);
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int r = (threadIdx.x >> 6) + u * (THR / WAVE);
+    tile[q.trans ? lane : r][q.trans ? r : lane] = v[u] / den * EX;
   }
   __syncthreads();
   char* X = q.ws + w.x + (int64_t)i0 * w.np * 4 + j0 * 4;
-  char* XT = q.ws + w.xt[0] + (int64_t)j0 * w.mp * 4 + i0 * 4;
+  char* XT = q.ws + w.xt(0) + (int64_t)j0 * w.mp * 4 + i0 * 4;
   for (int it = threadIdx.x; it < 512; it += THR) {
     const int r = it >> 3, g = it & 7;
     float v[8];
@@ -573,14 +580,14 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
   const int mt = w.mp / T, i0 = wg % mt * T, j0 = wg / mt * T;
   const int64_t la = (int64_t)w.mp * 4, lx = (int64_t)w.np * 4;
   f16v acc[S::FR][S::FC];
-  product<S>(ws + w.B + i0 * la, ws + w.xt[job.side] + j0 * la, la, w.mp / KSTEP, lds, acc);
+  product<S>(ws + w.B + i0 * la, ws + w.xt(job.side) + j0 * la, la, w.mp / KSTEP, lds, acc);
   parts_of<S>(acc, 1.f / EB, lds, [&](float* c, int pi, int pj, int thread) {
     const int i = i0 + pi, j = j0 + pj;
     char* X = ws + w.x + i * lx + (int64_t)j * 4;
     if (job.last)
       finish_out<SUB>(result, dtype, trans, m, n, c, X, job.a, lx, i, j, thread);
     else
-      finish<SUB, SUB>(c, X, job.a, 1.f, X, ws + w.xt[1 - job.side] + j * la + (int64_t)i * 4, lx, la, thread, THR);
+      finish<SUB, SUB>(c, X, job.a, 1.f, X, ws + w.xt(1 - job.side) + j * la + (int64_t)i * 4, lx, la, thread, THR);
   });
 }
 
