@@ -46,6 +46,7 @@ struct Mat {
   struct Cut {
     int32_t full, splits;  // whole tiles, pieces of k of the others
   } gram, poly;
+  int32_t sym;      // tile of the symmetric products
 };
 
 struct Job {
@@ -74,7 +75,7 @@ struct Parts {
     B = A + ab;
     norm = B + ab;
     split = norm + NORM_WGS * 8;
-    const int64_t st = T < 128 ? T : 128, nt = mp / st, tri = nt * (nt + 1) / 2;  // the symmetric products' tiles
+    const int64_t st = q.sym, nt = mp / st, tri = nt * (nt + 1) / 2;  // the symmetric products' tiles
     const auto cut = [&](const Mat::Cut& c) { return c.splits > 1 ? (tri - c.full) * c.splits * st * st * 4 : 0; };
     bytes = split + (cut(q.gram) > cut(q.poly) ? cut(q.gram) : cut(q.poly));
   }
@@ -592,12 +593,19 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
 }
 
 // ---------------------------------------------------------------------------------------- host
-// The tile of X: 256 from 192 of those on (a workgroup a CU), 128 from 192 of those on; below that tiles of 64
-// give four times the workgroups.  The symmetric products take tiles of at most 128 (256 would leave half of the
-// CUs idle at 4096).
+// The tile of X: 256 from 136 of those on, 128 from 192 of those on, else 64 (measured, five steps: 2048 x 4096,
+// 128 tiles of 256, 1,125 us in tiles of 128 and 1,266 of 256; 2900 x 2900, 144 tiles, 2,012 and 1,888; 1536 x 1536,
+// 144 tiles of 128, 589 us and 447 in 64; 2048 x 4096, 512 tiles, 1,125 and 1,229).
 int tile_of(const Mat& q) {
   const auto tiles = [&](int t) { return (int64_t)((q.m + t - 1) / t) * ((q.n + t - 1) / t); };
-  return tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+  return tiles(256) >= 136 ? 256 : tiles(128) >= 192 ? 128 : 64;
+}
+
+// The tile of the symmetric products, at most 128 (256 would leave half of the CUs idle at 4096): where X's is 128,
+// 64 up to 192 tiles of 128 (1024 x 4096, 36 tiles: 531 us in tiles of 128, 413 in 64; 2900 x 2900, 276: 2,012, 2,332).
+int sym_tile_of(const Mat& q, int tile) {
+  const int64_t nt = (q.m + 127) / 128;
+  return tile == 64 || (tile == 128 && nt * (nt + 1) / 2 <= 192) ? 64 : 128;
 }
 
 // Which tiles of a symmetric product over `steps` k-steps are cut along k.  Fewer than half of what the card
@@ -619,9 +627,8 @@ int layout(Job& job, F wgs_of) {
   return job.start[job.count];
 }
 
-template <int T>
+template <int T, int ST>
 int run_set(Job& job, int steps, hipStream_t st) {
-  constexpr int ST = T < 128 ? T : 128;
   int n = layout(job, [](const Mat& q) { return norm_parts((int64_t)q.m * q.n); });
   k_norm<T><<<n, THR, 0, st>>>(job);
   n = layout(job, [](const Mat& q) { return pad_to(q.m, T) / 64 * (pad_to(q.n, T) / 64); });
@@ -665,23 +672,24 @@ int to_mat(const regcn_matrix& d, Mat& q) {
   q.n = (int)std::max(d.rows, d.cols);
   q.dtype = d.dtype;
   if ((int64_t)q.m * q.n > (1ll << 40)) return set_error(REGCN_ENOTSUP, "orthogonalize: up to 2^40 elements");
-  const int t = tile_of(q), st = std::min(t, 128), nt = pad_to(q.m, t) / st, tri = nt * (nt + 1) / 2;
+  const int t = tile_of(q), st = q.sym = sym_tile_of(q, t), nt = pad_to(q.m, t) / st, tri = nt * (nt + 1) / 2;
   q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP);
   q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP);
   return 0;
 }
 
-// Matrices in sets: one tile size, at most MAXM.
+// Matrices in sets: one pair of tile sizes, at most MAXM.
 template <typename F>
 int for_sets(const regcn_matrix* mats, int count, F run) {
-  for (int tile = 64; tile <= 256; tile *= 2) {
+  constexpr int sets[4][2] = {{64, 64}, {128, 64}, {128, 128}, {256, 128}};
+  for (const auto& set : sets) {
     Job job{};
     for (int k = 0; k < count; ++k) {
       Mat q;
       if (int rc = to_mat(mats[k], q)) return rc;
-      if (tile_of(q) == tile) job.mat[job.count++] = q;
+      if (tile_of(q) == set[0] && q.sym == set[1]) job.mat[job.count++] = q;
       if (job.count == MAXM || (k == count - 1 && job.count)) {
-        if (int rc = run(job, tile)) return rc;
+        if (int rc = run(job, set[0])) return rc;
         job = Job{};
       }
     }
@@ -727,9 +735,9 @@ int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float
     job.b = b;
     job.c = c;
     job.eps = eps;
-    return tile == 256   ? run_set<256>(job, steps, st)
-           : tile == 128 ? run_set<128>(job, steps, st)
-                         : run_set<64>(job, steps, st);
+    if (tile == 256) return run_set<256, 128>(job, steps, st);
+    if (tile == 128) return job.mat[0].sym == 64 ? run_set<128, 64>(job, steps, st) : run_set<128, 128>(job, steps, st);
+    return run_set<64, 64>(job, steps, st);
   });
 }
 

@@ -89,7 +89,7 @@ def test_sizes(m, n, kind, dt):
     assert torch.equal(out, muon.orthogonalize(G))  # the same bits on every call
 
 
-@pytest.mark.parametrize("m,n", [(1700, 1701), (1921, 1600), (129, 30011), (3585, 3500), (500, 28001)])
+@pytest.mark.parametrize("m,n", [(1700, 1701), (1921, 1600), (129, 30011), (3585, 3500), (500, 28001), (2305, 2700)])
 def test_wide_tiles(m, n):
     """From 192 tiles of 128, and of 256, on: ragged sides, both orientations, k in pieces, a cut last round."""
     for kind in ("flat", "decay"):
