@@ -129,6 +129,9 @@ struct Cut {
   float s;
   int idx;
   __device__ bool keeps(float x, int i) const { return x > s || (x == s && i <= idx); }
+  // The shorter of two kept sets, of which `from` holds this one: a cut found among from's knows nothing of the
+  // equal scores that from leaves out.
+  __device__ Cut within(const Cut& from) const { return {s, s == from.s && from.idx < idx ? from.idx : idx}; }
 };
 
 // The weights of VE consecutive scores, 0 where a limit leaves one out.  No branch a score: the exponentials
@@ -375,7 +378,7 @@ __device__ __forceinline__ uint64_t draw_at(const RowArgs& a, int64_t at, uint64
 __device__ __forceinline__ void store_draw(const RowArgs& a, int64_t at, int id, float s, uint64_t sum, const Limits& l) {
   a.ids[at] = id;
   if (a.logp) {
-    const double log_sum = log((double)sum) - (double)l.shift * 0.69314718055994530942;
+    const double log_sum = log(__builtin_ldexp((double)sum, -l.shift));  // a sum of one weight 1: exactly 0
     a.logp[at] = (float)((s == l.top ? 0.0 : ((double)s - (double)l.top) * l.inv_t) - log_sum);
   }
 }
@@ -457,13 +460,14 @@ __device__ Cut find_cut(const LdsRow<THR>& row, Shared<THR>& sh, uint32_t kmin, 
     });
     __syncthreads();
     const int count = (int)sh.count;
-    if (count <= LIST) return order_list<WEIGHTS>(sh, count, above, target, l, c);
+    if (count <= LIST) return order_list<WEIGHTS>(sh, count, above, target, l, c).within(from);
     kmin = ALL - sh.lo_inv;
     kmax = sh.hi;
     __syncthreads();
   }
   return descend_cut<WEIGHTS>(Among<LdsRow<THR>>{row, from}, sh, kmin, kmax, above, cols, l, c,
-                              [&](uint64_t total) { return target ? target : target_of(total); });
+                              [&](uint64_t total) { return target ? target : target_of(total); })
+      .within(from);
 }
 
 template <typename T, int THR, int MAX>
@@ -758,7 +762,7 @@ __global__ __launch_bounds__(1024) void k_spread_cut(Spread p) {
     const uint32_t lo = ready ? ALL - st.lo_inv[WEIGHTS] : ALL - st.kmin_inv, hi = ready ? st.hi[WEIGHTS] : st.kmax;
     cut = descend_cut<WEIGHTS>(all, sh, lo, hi, ready ? st.above[WEIGHTS] : 0, p.a.cols, l, p.a.c, target_of);
   }
-  if (threadIdx.x == 0) st.cut[WEIGHTS] = cut;
+  if (threadIdx.x == 0) st.cut[WEIGHTS] = cut.within(from);
 }
 
 // The row's last cut and its limits, min_p among them.

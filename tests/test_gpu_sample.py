@@ -119,7 +119,8 @@ def test_ties(N):
     s[1] = torch.randint(0, 3, (N,)).float()
     s[2, : N // 2] = 4.0
     s[3] = torch.where(torch.arange(N) % 2 == 0, torch.zeros(N), -torch.zeros(N))  # 0 and -0 are equal
-    for lim in (dict(k=17), dict(p=0.5), dict(p=0.37), dict(k=N // 3, p=0.61), dict(k=N // 2 + 1), dict(m=0.2, k=9)):
+    for lim in (dict(k=17), dict(p=0.5), dict(p=0.37), dict(k=N // 3, p=0.61), dict(k=N // 2 + 1), dict(m=0.2, k=9),
+                dict(k=1, p=0.9), dict(k=2, p=0.99), dict(k=N - 1, p=0.999)):
         check(s, u, **lim)
     # keeping only the first 17 ids of a constant row, evenly spaced numbers take each of them
     even = ((torch.arange(17, dtype=torch.float64) + 0.5) / 17).to(DEV)
@@ -134,6 +135,14 @@ def test_numbers_at_the_ends():
     assert (got[:, 5] == 0).all() and (got[:, 6] == 0).all()
     f = torch.rand(3, 2, device=DEV)
     assert torch.equal(ranking.sample(s, f), ranking.sample(s, f.double()))
+
+
+@pytest.mark.parametrize("N", [1, 700, 50000])
+def test_a_certain_draw_has_log_probability_zero(N):
+    s, u = make(3, N, 2, 6)
+    for lim in (dict(top_k=1), dict(temperature=0.0), dict(top_p=0.0), dict(min_p=1.0)):
+        ids, logp = ranking.sample(s, u, return_logp=True, **lim)
+        assert torch.equal(ids, s.argmax(1, keepdim=True).expand(3, 2)) and not bool(logp.any())
 
 
 @pytest.mark.parametrize("N", [500, 40000])
@@ -178,6 +187,18 @@ def test_strides_and_shapes():
 def test_many_rows_and_draws():
     s, u = make(700, 1000, 33, 13)
     check(s, u, T=0.9, k=200, p=0.95)
+
+
+@pytest.mark.parametrize("N", [3000, 60000])
+@pytest.mark.parametrize("k", [1, 2, 3, 40])
+def test_equal_scores_at_the_top(N, k):
+    """Several scores share the top: top_k leaves some of them out, and top_p must not let them in again."""
+    s, u = make(6, N, 5, k, BF16)
+    top = float(s.float().max()) + 1.0
+    for r, n in enumerate((2, 2, 3, 5, 100, 700)):
+        s[r, torch.randperm(N, generator=torch.Generator().manual_seed(r))[:n].to(DEV)] = top
+    for lim in (dict(), dict(p=0.93), dict(p=0.999999), dict(p=0.4), dict(m=0.5)):
+        check(s, u, k=k, **lim)
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
