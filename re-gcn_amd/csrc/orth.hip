@@ -15,7 +15,12 @@
 // subnormal halves as they are.  E is 12 for X and A and 11 for B: the binding refuses coefficients whose
 // iteration leaves |s| <= 2 or |b s^2 + c s^4| <= 16, so nothing passes 2^15.
 //
-// Layout of an operand: rows of 8-element groups, each group 8 hi then 8 lo halves: a tile's k-step of
+// Matrices of up to 64 rows (or columns) stay in fp32 and use the fp32 matrix instruction: their few singular values
+// leave little to average errors out, and 3 x 30 in halves was off by 1 to 4.5e-6 of its norm after five steps where
+// fp32 is by 0.3 to 1.4e-6; from 100 x 200 on halves are the closer ones (200 x 200: 1.2e-6, 1.6e-6).  Their
+// products are short, so it costs little: 3 x 30 71 -> 75 us, 64 x 1024 107 -> 136, 64 x 10000 139 -> 148.
+//
+// Layout of an operand: rows of 8-element groups, each group 8 hi then 8 lo halves (or 8 fp32): a tile's k-step of
 // 32 is one 128-byte line of a row.  Rows and columns are padded to the tile with zeros, which
 // stay zero through every product, so the inner loop has no bounds.
 //
@@ -134,8 +139,16 @@ __global__ __launch_bounds__(THR) void k_norm(Job job) {
   if (threadIdx.x == 0) ((double*)(q.ws + Parts<T>(q).norm))[wg] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-// 8 numbers as a group: 8 hi, 8 lo.
-__device__ __forceinline__ void store_group(char* p, const float (&v)[8]) {
+// A matrix held in fp32: its tile is 64 and it is one row of tiles.
+__host__ __device__ inline bool in_fp32(const Mat& q, int tile) { return tile == 64 && q.m <= 64; }
+
+// 8 numbers as a group: 8 hi, 8 lo, or 8 fp32.
+__device__ __forceinline__ void store_group(char* p, const float (&v)[8], bool fp32) {
+  if (fp32) {
+    reinterpret_cast<f4*>(p)[0] = f4{v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f4*>(p)[1] = f4{v[4], v[5], v[6], v[7]};
+    return;
+  }
   h8 hi, lo;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -146,7 +159,16 @@ __device__ __forceinline__ void store_group(char* p, const float (&v)[8]) {
   reinterpret_cast<h8*>(p)[1] = lo;
 }
 
-__device__ __forceinline__ void load_group(float (&v)[8], const char* p) {
+__device__ __forceinline__ void load_group(float (&v)[8], const char* p, bool fp32) {
+  if (fp32) {
+    const f4 a = reinterpret_cast<const f4*>(p)[0], b = reinterpret_cast<const f4*>(p)[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+    return;
+  }
   const h8 hi = reinterpret_cast<const h8*>(p)[0], lo = reinterpret_cast<const h8*>(p)[1];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
@@ -197,10 +219,10 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[r][8 * g + e];
-    store_group(X + (int64_t)r * w.np * 4 + g * 32, v);
+    store_group(X + (int64_t)r * w.np * 4 + g * 32, v, in_fp32(q, T));
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[8 * g + e][r];
-    store_group(XT + (int64_t)r * w.mp * 4 + g * 32, v);
+    store_group(XT + (int64_t)r * w.mp * 4 + g * 32, v, in_fp32(q, T));
   }
 }
 
@@ -238,7 +260,9 @@ __device__ __forceinline__ void load_lds(char* base, int voff, int soff, char* d
 // the other's are read, and in the second half the next stage's first.  The barrier stands between
 // the halves: behind it every wave has read all of stage k, whose place the loads of stage k + STAGES take, and
 // stage k + 1 has landed.  So neither an LDS read nor a load is waited for right after its issue.
-template <typename S>
+//
+// FP32: the operands hold fp32 numbers and each of the 8 k of a group is a product of its own, two groups at a time.
+template <typename S, bool FP32>
 __device__ __forceinline__ void product(const char* __restrict__ p, const char* __restrict__ q, int64_t ld, int steps,
                                         char* lds, f16v (&acc)[S::FR][S::FC]) {
   constexpr int T = S::T;
@@ -279,6 +303,16 @@ __device__ __forceinline__ void product(const char* __restrict__ p, const char* 
     for (int i = 0; i < S::FR; ++i) f.al[i] = *reinterpret_cast<const h8*>(st + swizzle(wr, g + 1) + i * 4096);
   };
   const auto multiply = [&](const Half& f) {
+    if constexpr (FP32) {
+      static_assert(S::FR == 1 && S::FC == 1, "one fragment of 32 x 32 a wave");
+      const f4 a0 = __builtin_bit_cast(f4, f.ah[0]), a1 = __builtin_bit_cast(f4, f.al[0]);
+      const f4 b0 = __builtin_bit_cast(f4, f.bh[0]), b1 = __builtin_bit_cast(f4, f.bl[0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0[e], b0[e], acc[0][0], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a1[e], b1[e], acc[0][0], 0, 0, 0);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < S::FR; ++i)
 #pragma unroll
@@ -309,7 +343,7 @@ __device__ __forceinline__ void product(const char* __restrict__ p, const char* 
   Half even, odd;
   read(even, lds, 0);
   // reads, loads and products interleaved one by one, so that the matrix cores never wait for a run of issues
-  constexpr int NM = 3 * S::FR * S::FC, NR = 2 * (S::FR + S::FC), NL = S::LOADS;
+  constexpr int NM = (FP32 ? 8 : 3) * S::FR * S::FC, NR = 2 * (S::FR + S::FC), NL = S::LOADS;
   int at = 0, next = S::STAGE;  // stage k, stage k + 1
   for (int k = 0; k < last; ++k) {
     read(odd, lds + at, 1);
@@ -344,6 +378,16 @@ __device__ __forceinline__ void product(const char* __restrict__ p, const char* 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the end, before the stages become the tile
 }
 
+// The same in the matrix's own form.
+template <typename S>
+__device__ __forceinline__ void product_of(bool fp32, const char* __restrict__ p, const char* __restrict__ q, int64_t ld,
+                                           int steps, char* lds, f16v (&acc)[S::FR][S::FC]) {
+  if constexpr (S::T == 64) {
+    if (fp32) return product<S, true>(p, q, ld, steps, lds, acc);
+  }
+  product<S, false>(p, q, ld, steps, lds, acc);
+}
+
 // The tile through LDS in parts: f(c, i, j, thread) for each SUB x SUB part at row i, column j of the tile, its
 // products (times `unscale`) in c, by 256 threads.
 template <typename S, typename F>
@@ -376,20 +420,20 @@ __device__ __forceinline__ void parts_of(const f16v (&acc)[S::FR][S::FC], float 
 // stored as operand rows at `dst` and, transposed, at `dst_t` (null: not stored), both at the part's corner.
 // One barrier of the workgroup.
 template <int RW, int CL>
-__device__ __forceinline__ void finish(float* c, const char* old, float alpha, float beta, char* dst, char* dst_t,
+__device__ __forceinline__ void finish(bool fp32, float* c, const char* old, float alpha, float beta, char* dst, char* dst_t,
                                        int64_t ld, int64_t ld_t, int thread, int threads) {
   constexpr int G = CL / 8, LD = CL + 1;
   for (int it = thread; it < RW * G; it += threads) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
-    if (old) load_group(x, old + r * ld + g * 32);
+    if (old) load_group(x, old + r * ld + g * 32, fp32);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e] = beta * c[r * LD + 8 * g + e];
       if (old) v[e] = fmaf(alpha, x[e], v[e]);
       c[r * LD + 8 * g + e] = v[e];
     }
-    if (dst) store_group(dst + r * ld + g * 32, v);
+    if (dst) store_group(dst + r * ld + g * 32, v, fp32);
   }
   __syncthreads();
   if (!dst_t) return;
@@ -399,7 +443,7 @@ __device__ __forceinline__ void finish(float* c, const char* old, float alpha, f
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = c[(8 * g + e) * LD + col];
-    store_group(dst_t + col * ld_t + g * 32, v);
+    store_group(dst_t + col * ld_t + g * 32, v, fp32);
   }
 }
 
@@ -424,13 +468,13 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t at, cons
 
 // The last step's tile into the result, in G's type and orientation.
 template <int T>
-__device__ __forceinline__ void finish_out(void* out, int dtype, bool trans, int m, int n, float* c, const char* old,
+__device__ __forceinline__ void finish_out(bool fp32, void* out, int dtype, bool trans, int m, int n, float* c, const char* old,
                                            float alpha, int64_t ld, int i0, int j0, int thread) {
   constexpr int G = T / 8;
   for (int it = thread; it < T * G; it += THR) {
     const int r = it / G, g = it % G;
     float v[8], x[8];
-    load_group(x, old + r * ld + g * 32);
+    load_group(x, old + r * ld + g * 32, fp32);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e] = fmaf(alpha, x[e], c[r * (T + 1) + 8 * g + e]) * (1.f / EX);
@@ -472,7 +516,7 @@ __device__ __forceinline__ Piece2 symmetric_piece(int wg, int nt, int full, int 
 // alpha old + beta P P^T of one tile of the upper triangle, both halves stored; or one piece of k of it, stored as
 // fp32 partial sums.
 template <typename S>
-__device__ __forceinline__ void symmetric(const Piece2& at, int splits, const char* P, int64_t ld, int steps, const char* old,
+__device__ __forceinline__ void symmetric(bool fp32, const Piece2& at, int splits, const char* P, int64_t ld, int steps, const char* old,
                                           float alpha, float beta, char* out, int64_t la, float* part, int64_t cut,
                                           char* lds) {
   constexpr int T = S::T;
@@ -480,14 +524,14 @@ __device__ __forceinline__ void symmetric(const Piece2& at, int splits, const ch
   const int k0 = at.t < 0 ? 0 : (int)((int64_t)steps * at.s / splits);
   const int k1 = at.t < 0 ? steps : (int)((int64_t)steps * (at.s + 1) / splits);
   f16v acc[S::FR][S::FC];
-  product<S>(P + (int64_t)at.i * T * ld + k0 * 128, P + (int64_t)at.j * T * ld + k0 * 128, ld, k1 - k0, lds, acc);
+  product_of<S>(fp32, P + (int64_t)at.i * T * ld + k0 * 128, P + (int64_t)at.j * T * ld + k0 * 128, ld, k1 - k0, lds, acc);
   parts_of<S>(acc, 1.f, lds, [&](float* c, int, int, int thread) {
     if (at.t >= 0) {
       float* to = part + (at.s * cut + at.t) * T * T;
       for (int it = thread; it < T * T; it += THR) to[it] = c[it / T * (T + 1) + it % T];
       return;
     }
-    finish<T, T>(c, old ? old + at.i * T * la + at.j * T * 4 : nullptr, alpha, beta, out + at.i * T * la + at.j * T * 4,
+    finish<T, T>(fp32, c, old ? old + at.i * T * la + at.j * T * 4 : nullptr, alpha, beta, out + at.i * T * la + at.j * T * 4,
               at.i == at.j ? nullptr : out + at.j * T * la + at.i * T * 4, la, la, thread, THR);
   });
 }
@@ -496,7 +540,7 @@ __device__ __forceinline__ void symmetric(const Piece2& at, int splits, const ch
 // columns, its pieces' loads under way together.
 constexpr int STRIP = 32;
 template <int T>
-__device__ __forceinline__ void symmetric_sum(int wg, int nt, int full, int splits, const float* part, const char* old,
+__device__ __forceinline__ void symmetric_sum(bool fp32, int wg, int nt, int full, int splits, const float* part, const char* old,
                                               float alpha, float beta, char* out, int64_t la, float* c) {
   int i, j;
   const int t = wg / (T / STRIP), r0 = wg % (T / STRIP) * STRIP;
@@ -513,7 +557,7 @@ __device__ __forceinline__ void symmetric_sum(int wg, int nt, int full, int spli
   }
   __syncthreads();
   const int64_t at = (int64_t)(i * T + r0) * la + j * T * 4;
-  finish<STRIP, T>(c, old ? old + at : nullptr, alpha, beta, out + at,
+  finish<STRIP, T>(fp32, c, old ? old + at : nullptr, alpha, beta, out + at,
                    i == j ? nullptr : out + j * T * la + (i * T + r0) * 4, la, la, threadIdx.x, THR);
 }
 
@@ -526,7 +570,7 @@ __global__ __launch_bounds__(THR, 2) void k_gram(Job job) {
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
   const int nt = w.mp / T;
-  symmetric<S>(symmetric_piece(wg, nt, q.gram.full, q.gram.splits), q.gram.splits, q.ws + w.x, (int64_t)w.np * 4,
+  symmetric<S>(in_fp32(q, PAD), symmetric_piece(wg, nt, q.gram.full, q.gram.splits), q.gram.splits, q.ws + w.x, (int64_t)w.np * 4,
                w.np / KSTEP, nullptr, 0.f, 1.f / EX, q.ws + w.A, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
                nt * (nt + 1) / 2 - q.gram.full, lds);
 }
@@ -536,7 +580,7 @@ __global__ __launch_bounds__(THR) void k_gram_sum(Job job) {
   int wg = blockIdx.x;
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
-  symmetric_sum<T>(wg, w.mp / T, q.gram.full, q.gram.splits, (const float*)(q.ws + w.split), nullptr, 0.f, 1.f / EX,
+  symmetric_sum<T>(in_fp32(q, PAD), wg, w.mp / T, q.gram.full, q.gram.splits, (const float*)(q.ws + w.split), nullptr, 0.f, 1.f / EX,
                    q.ws + w.A, (int64_t)w.mp * 4, c);
 }
 
@@ -550,7 +594,7 @@ __global__ __launch_bounds__(THR, 2) void k_poly(Job job) {
   const Parts<PAD> w(q);
   const int nt = w.mp / T;
   const char* A = q.ws + w.A;
-  symmetric<S>(symmetric_piece(wg, nt, q.poly.full, q.poly.splits), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
+  symmetric<S>(in_fp32(q, PAD), symmetric_piece(wg, nt, q.poly.full, q.poly.splits), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
                job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
                nt * (nt + 1) / 2 - q.poly.full, lds);
 }
@@ -560,7 +604,7 @@ __global__ __launch_bounds__(THR) void k_poly_sum(Job job) {
   int wg = blockIdx.x;
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
-  symmetric_sum<T>(wg, w.mp / T, q.poly.full, q.poly.splits, (const float*)(q.ws + w.split), q.ws + w.A,
+  symmetric_sum<T>(in_fp32(q, PAD), wg, w.mp / T, q.poly.full, q.poly.splits, (const float*)(q.ws + w.split), q.ws + w.A,
                    job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, c);
 }
 
@@ -577,27 +621,28 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
   char* const ws = q.ws;
   void* const result = q.out;
   const int m = q.m, n = q.n, dtype = q.dtype;
-  const bool trans = q.trans;
+  const bool trans = q.trans, fp32 = in_fp32(q, T);
   const int mt = w.mp / T, i0 = wg % mt * T, j0 = wg / mt * T;
   const int64_t la = (int64_t)w.mp * 4, lx = (int64_t)w.np * 4;
   f16v acc[S::FR][S::FC];
-  product<S>(ws + w.B + i0 * la, ws + w.xt(job.side) + j0 * la, la, w.mp / KSTEP, lds, acc);
+  product_of<S>(fp32, ws + w.B + i0 * la, ws + w.xt(job.side) + j0 * la, la, w.mp / KSTEP, lds, acc);
   parts_of<S>(acc, 1.f / EB, lds, [&](float* c, int pi, int pj, int thread) {
     const int i = i0 + pi, j = j0 + pj;
     char* X = ws + w.x + i * lx + (int64_t)j * 4;
     if (job.last)
-      finish_out<SUB>(result, dtype, trans, m, n, c, X, job.a, lx, i, j, thread);
+      finish_out<SUB>(fp32, result, dtype, trans, m, n, c, X, job.a, lx, i, j, thread);
     else
-      finish<SUB, SUB>(c, X, job.a, 1.f, X, ws + w.xt(1 - job.side) + j * la + (int64_t)i * 4, lx, la, thread, THR);
+      finish<SUB, SUB>(fp32, c, X, job.a, 1.f, X, ws + w.xt(1 - job.side) + j * la + (int64_t)i * 4, lx, la, thread, THR);
   });
 }
 
 // ---------------------------------------------------------------------------------------- host
-// The tile of X: 256 from 136 of those on, 128 from 192 of those on, else 64 (measured, five steps: 2048 x 4096,
+// The tile of X: 256 from 136 of those on, 128 from 192 of those on, else 64, and none that fewer rows than half of it
+// would fill.  Measured, five steps: 64 x 40000 542 us in tiles of 256, 232 in 64; 128 x 40000 545, and 264 in 128; 2048 x 4096,
 // 128 tiles of 256, 1,125 us in tiles of 128 and 1,266 of 256; 2900 x 2900, 144 tiles, 2,012 and 1,888; 1536 x 1536,
-// 144 tiles of 128, 589 us and 447 in 64; 2048 x 4096, 512 tiles, 1,125 and 1,229).
+// 144 tiles of 128, 589 us and 447 in 64; 2048 x 4096, 512 tiles, 1,125 and 1,229.
 int tile_of(const Mat& q) {
-  const auto tiles = [&](int t) { return (int64_t)((q.m + t - 1) / t) * ((q.n + t - 1) / t); };
+  const auto tiles = [&](int t) { return q.m > t / 2 ? (int64_t)((q.m + t - 1) / t) * ((q.n + t - 1) / t) : 0; };
   return tiles(256) >= 136 ? 256 : tiles(128) >= 192 ? 128 : 64;
 }
 
@@ -610,12 +655,12 @@ int sym_tile_of(const Mat& q, int tile) {
 
 // Which tiles of a symmetric product over `steps` k-steps are cut along k.  Fewer than half of what the card
 // holds (two workgroups a CU): cut into pieces of at least 24 k-steps (about 6 us; the second launch that adds them
-// up costs 4).  More: a last round that fills less than half of it is cut (4096: 16 of 528 tiles; 280 -> 220 us).
-Mat::Cut cut_of(int tri, int steps) {
+// up costs 4), 12 in fp32.  More: a last round that fills less than half of it is cut (4096: 16 of 528 tiles; 280 -> 220 us).
+Mat::Cut cut_of(int tri, int steps, bool fp32) {
   const int slots = 512, rest = tri % slots;
   const int full = tri - rest;
   if (rest == 0 || rest > slots / 2) return {tri, 1};
-  const int splits = full ? std::min({slots / rest, steps / 8, 8}) : std::min({slots / rest, steps / 24, 32});
+  const int splits = full ? std::min({slots / rest, steps / 8, 8}) : std::min({slots / rest, steps / (fp32 ? 12 : 24), fp32 ? 64 : 32});
   if (splits < 2) return {tri, 1};
   return {full, splits};
 }
@@ -673,8 +718,8 @@ int to_mat(const regcn_matrix& d, Mat& q) {
   q.dtype = d.dtype;
   if ((int64_t)q.m * q.n > (1ll << 40)) return set_error(REGCN_ENOTSUP, "orthogonalize: up to 2^40 elements");
   const int t = tile_of(q), st = q.sym = sym_tile_of(q, t), nt = pad_to(q.m, t) / st, tri = nt * (nt + 1) / 2;
-  q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP);
-  q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP);
+  q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP, in_fp32(q, t));
+  q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP, in_fp32(q, t));
   return 0;
 }
 

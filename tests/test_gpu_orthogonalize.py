@@ -97,6 +97,16 @@ def test_wide_tiles(m, n):
         check(muon.orthogonalize(G), G)
 
 
+@pytest.mark.parametrize("m,n", [(1, 300000), (3, 30), (64, 1024), (32, 100003), (50001, 64), (65, 40000), (40000, 128)])
+def test_few_rows(m, n):
+    """Up to 64 rows (held in fp32) and just above, however long they are; a set that holds both."""
+    G = [matrix(m, n, s) for s in (1, 2)] + [matrix(100, 90, 3)]
+    together = muon.orthogonalize(G)
+    for g, o in zip(G, together):
+        check(o, g)
+        assert torch.equal(o, muon.orthogonalize(g))
+
+
 @pytest.mark.parametrize("steps,coeffs", [(1, muon.COEFFS), (2, muon.COEFFS), (8, muon.COEFFS), (5, (1.5, -0.5, 0.0)),
                                           (12, (1.875, -1.25, 0.375))])
 def test_steps_and_coefficients(steps, coeffs):
