@@ -190,7 +190,7 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
   for (int p = lane; p < parts; p += WAVE) s += part[p];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  const float den = (float)sqrt(s) + job.eps;
+  const double inv = 1.0 / (sqrt(s) + (double)job.eps);  // in 64 bits: the norm of finite numbers may pass the fp32 range
   const int nt = w.np / 64, i0 = wg / nt * 64, j0 = wg % nt * 64;
   const int rows = q.trans ? q.n : q.m, cols = q.trans ? q.m : q.n;  // as stored
   const int r0 = q.trans ? j0 : i0, c0 = q.trans ? i0 : j0;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int r = (threadIdx.x >> 6) + u * (THR / WAVE);
-    tile[q.trans ? lane : r][q.trans ? r : lane] = v[u] / den * EX;
+    tile[q.trans ? lane : r][q.trans ? r : lane] = (float)(v[u] * inv) * EX;
   }
   __syncthreads();
   char* X = q.ws + w.x + (int64_t)i0 * w.np * 4 + j0 * 4;

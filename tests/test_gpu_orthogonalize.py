@@ -149,6 +149,15 @@ def test_range_of_the_input(scale):
     check(muon.orthogonalize(G, eps=0.0), G, eps=0.0)
 
 
+def test_norm_past_the_range_of_fp32():
+    """Finite entries whose norm is not an fp32 number."""
+    for m, n in ((60, 80), (300, 200)):
+        G = matrix(m, n, 5) * 4e39
+        assert bool(torch.isfinite(G).all())
+        assert float(G.double().norm()) > 3.5e38
+        check(muon.orthogonalize(G), G)
+
+
 def test_zero_and_not_finite():
     zero = torch.zeros(70, 30, device=DEV)
     bad = matrix(40, 40, 1).clone()
