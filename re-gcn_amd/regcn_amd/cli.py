@@ -488,6 +488,10 @@ def main(argv=None):
         raise ValueError("--radius-anchor-beta must be in [0, 1]")
     if args.sample_draws < 0:
         raise ValueError("--sample-draws must be non-negative (0: the --topk best)")
+    if not (0.0 <= args.sample_temperature < float("inf") and args.sample_top_k >= 0 and 0.0 <= args.sample_top_p <= 1.0
+            and 0.0 <= args.sample_min_p <= 1.0):
+        raise ValueError("--sample-temperature and --sample-top-k must be non-negative, --sample-top-p and "
+                         "--sample-min-p in [0, 1]")
     if args.gpu < 0 or not torch.cuda.is_available():
         raise SystemExit("the HIP path needs a GPU (--gpu N); there is no CPU fallback")
     world = int(os.environ.get("WORLD_SIZE", "1"))

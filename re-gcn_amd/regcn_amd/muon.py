@@ -50,7 +50,7 @@ def _plan(g):
 def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7):
     """Newton-Schulz orthogonalisation of a matrix (m x n), of a stack of them (... x m x n), or of a list
     or tuple of matrices of any shapes and types on one device; the same structure is returned, each result
-    in its matrix's type.  An all-zero matrix stays zero, a matrix without elements is returned as it is;
+    in its matrix's type.  An all-zero matrix stays zero (with an eps of 0 it becomes NaN), a matrix without elements is returned as it is;
     infinities and NaN make their matrix's result NaN.  No gradient flows through the iteration."""
     steps = int(steps)
     if not 1 <= steps <= 1000:
@@ -104,7 +104,8 @@ class Muon(torch.optim.Optimizer):
         d = grad + momentum * buf          (nesterov; otherwise buf)
         p = (1 - lr * weight_decay) * p - lr * sqrt(max(1, rows / cols)) * orthogonalize(d)
 
-    One call of `orthogonalize` serves all the parameters of a group (per device).  Parameters without a
+    One call of `orthogonalize` serves all the parameters of a group (per device).  The momentum and the step
+    are fp32 whatever the parameter's type: a 16-bit parameter is rounded once, at the end.  Parameters without a
     gradient are left alone; sparse gradients are refused.  The step holds no host synchronisation, so a
     training step with it can be captured in a HIP graph (training.GraphedSteps)."""
 
@@ -130,6 +131,15 @@ class Muon(torch.optim.Optimizer):
                 raise ValueError("Muon takes two-dimensional fp32, bf16 or fp16 parameters (got %s %s)"
                                  % (tuple(p.shape), p.dtype))
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts a state to its parameter's type; the momentum stays fp32
+        keys = [k for g in state_dict["param_groups"] for k in g["params"]]
+        for k, p in zip(keys, (p for g in self.param_groups for p in g["params"])):
+            if k in state_dict["state"]:
+                self.state[p]["momentum_buffer"] = state_dict["state"][k]["momentum_buffer"].to(
+                    device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -152,7 +162,7 @@ class Muon(torch.optim.Optimizer):
         for p in ps:
             st = self.state[p]
             if "momentum_buffer" not in st:
-                st["momentum_buffer"] = torch.zeros_like(p)
+                st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
             bufs.append(st["momentum_buffer"])
         mu, lr = group["momentum"], group["lr"]
         torch._foreach_mul_(bufs, mu)
@@ -163,9 +173,13 @@ class Muon(torch.optim.Optimizer):
             torch._foreach_add_(d, grads)
         o = orthogonalize(d, group["steps"], group["coeffs"], group["eps"])
         torch._foreach_mul_(o, [max(1.0, p.shape[0] / p.shape[1]) ** 0.5 if p.numel() else 1.0 for p in ps])
+        w = [p if p.dtype == torch.float32 else p.float() for p in ps]
         if group["weight_decay"]:
-            torch._foreach_mul_(ps, 1.0 - lr * group["weight_decay"])
-        torch._foreach_add_(ps, o, alpha=-lr)
+            torch._foreach_mul_(w, 1.0 - lr * group["weight_decay"])
+        torch._foreach_add_(w, o, alpha=-lr)
+        for p, x in zip(ps, w):
+            if x is not p:
+                p.copy_(x)
 
 
 TABLES = ("dynamic_emb", "emb_rel")  # rows looked up by id: not matrices of a product

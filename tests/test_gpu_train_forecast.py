@@ -105,6 +105,32 @@ def test_muon_step_against_the_formula(nesterov):
         assert torch.equal(again.state[p]["momentum_buffer"], opt.state[p]["momentum_buffer"])
 
 
+@pytest.mark.parametrize("dt,half_step", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_muon_step_of_16_bit_parameters(dt, half_step):
+    """The momentum and the step are fp32, the parameter is rounded once: half a step of its type, beside the
+    1e-5 of the update's norm that the fp32 step is allowed."""
+    g = torch.Generator().manual_seed(1)
+    p = torch.randn(40, 64, generator=g).to(DEV).to(dt).requires_grad_(True)
+    opt = muon.Muon([p], lr=0.05, momentum=0.9, weight_decay=0.1)
+    buf = torch.zeros(40, 64, dtype=torch.float64)
+    for step in range(4):
+        p.grad = (torch.randn(40, 64, generator=g) * 0.01).to(DEV).to(dt)
+        gr = p.grad.cpu().double()
+        buf.mul_(0.9).add_(gr)
+        want = p.detach().cpu().double() * (1 - 0.05 * 0.1) - 0.05 * _ortho64(gr + 0.9 * buf)
+        opt.step()
+        off = (p.detach().cpu().double() - want).abs()
+        assert float((off - half_step * 1.01 * want.abs()).max()) <= 1e-5 * 0.05 * 64 ** 0.5
+        m = opt.state[p]["momentum_buffer"]
+        assert m.dtype == torch.float32
+        assert float((m.cpu().double() - buf).abs().max()) <= 2 * (step + 1) * 2.0 ** -24 * 0.5
+        if step == 1:  # a resumed run goes on with the same bits
+            again = muon.Muon([p], lr=0.05, momentum=0.9, weight_decay=0.1)
+            again.load_state_dict(opt.state_dict())
+            assert torch.equal(again.state[p]["momentum_buffer"], m) and again.state[p]["momentum_buffer"].dtype == m.dtype
+            opt = again
+
+
 def test_split_parameters():
     model, _ = _model(_args())
     mats, rest = muon.split_parameters(model)
