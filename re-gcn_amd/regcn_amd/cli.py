@@ -151,9 +151,9 @@ class Optimizers:
     def __init__(self, *optimizers):
         self.optimizers = optimizers
 
-    def zero_grad(self):
+    def zero_grad(self, set_to_none=True):
         for o in self.optimizers:
-            o.zero_grad()
+            o.zero_grad(set_to_none)
 
     def step(self):
         for o in self.optimizers:
