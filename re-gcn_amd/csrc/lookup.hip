@@ -23,7 +23,7 @@
 namespace regcn {
 namespace {
 
-constexpr int RANK_MAX = 8192;     // tokens ranked by counting (their keys in 32 KB of LDS)
+constexpr int RANK_MAX = 8192;     // tokens ranked by counting (their keys in 32 KB of LDS; two workgroups a CU)
 constexpr int FAN = 16, LEVELS = 5;  // the tree of partial sums: 16, 256, 4096, 65536 tokens a node
 constexpr int RADIX_BITS = 10, BINS = 1 << RADIX_BITS;
 constexpr int MAX_TILES = 256;     // radix tiles (a workgroup each)
@@ -34,6 +34,7 @@ constexpr int ROW_THR = 256;
 // a 268 MB gradient 75 -> 59 us).  Smaller ones stay cached for the kernel that reads them next.
 constexpr int64_t STREAM_BYTES = 16 << 20;
 constexpr int MAX_ROWS = 512;      // rows a workgroup of k_row_grads
+constexpr int DEAL = 32;           // workgroups that share out their rows
 constexpr int SLICE = 16;          // 16-byte pieces of the columns a workgroup of k_partials takes
 
 struct Tokens {
@@ -82,7 +83,8 @@ __device__ __forceinline__ void clear_runs(int2* runs, int64_t V) {
 
 // One launch for n <= RANK_MAX: a workgroup ranks 64 tokens, each of its 16 waves counting a
 // sixteenth of the keys: rank = #{key_j < key} + #{j < i, key_j = key}.  n^2 compares spread over
-// the card: 16 million (n = 4096) take about 2 us, against 3 dependent sort passes on one CU.
+// the card: 7.5 us at 3,080 tokens, 10.9 at 4,999, 14.4 at 8,192 and 25 at 16,384, where two radix passes take 28
+// and grow with n only.
 __global__ __launch_bounds__(SORT_THR) void k_rank(Tokens t, int32_t* __restrict__ perm, uint32_t* __restrict__ skey,
                                                    int2* __restrict__ runs) {
   __shared__ __align__(16) uint32_t keys[RANK_MAX];
@@ -317,22 +319,31 @@ __global__ __launch_bounds__(ROW_THR) void k_partials(const T* __restrict__ g, c
 }
 
 // Every row of dtable, once: s times the sum of its run of sorted tokens, taken as the run's ends at
-// each level and the nodes between them; zero for a row without tokens.
+// each level and the nodes between them; zero for a row without tokens.  Frequent
+// rows often lie side by side, and a wave sums its rows one after the other: so every DEAL workgroups share out
+// their rows in groups of 2^grp, a wave's pieces and, where the output goes past the caches, whole 128-byte lines
+// (50,000 x 512 bf16, 8,192 tokens of Zipf exponent 1.2: 90 us with a workgroup's rows in one piece, 50 dealt; without
+// whole lines a 1,000,000 x 200 fp32 gradient took 361 us for 322).
 template <typename T>
 __global__ __launch_bounds__(ROW_THR) void k_row_grads(const T* __restrict__ g, const int32_t* __restrict__ perm,
                                                        const int2* __restrict__ runs, Levels lv, int64_t V, int d,
-                                                       int64_t dp, int rows_per_wg, float scale, bool stream_out,
+                                                       int64_t dp, int rows, int grp, float scale, bool stream_out,
                                                        T* __restrict__ out) {
   constexpr int VE = Piece<T>::VE;
   const int C = (d + VE - 1) / VE;
-  const int64_t v0 = (int64_t)blockIdx.x * rows_per_wg;
-  const int rows = (int)min((int64_t)rows_per_wg, V - v0);
+  const int64_t first = ((int64_t)(blockIdx.x / DEAL) * DEAL * (rows >> grp) + blockIdx.x % DEAL) << grp;
+  const auto row_of = [&](int r) { return first + ((r >> grp) * DEAL << grp) + (r & ((1 << grp) - 1)); };
   __shared__ int2 lrun[MAX_ROWS];  // one wait for all the rows' runs, then stores without loads for empty rows
-  for (int r = threadIdx.x; r < rows; r += ROW_THR) lrun[r] = runs[v0 + r];
+  for (int r = threadIdx.x; r < rows; r += ROW_THR) {
+    const int64_t v = row_of(r);
+    if (v < V) lrun[r] = runs[v];
+  }
   __syncthreads();
   for (int it = threadIdx.x; it < rows * C; it += ROW_THR) {
     const int r = (int)((uint32_t)it / (uint32_t)C);
     const int c0 = (it - r * C) * VE, m = d - c0;
+    const int64_t v = row_of(r);
+    if (v >= V) continue;
     const int2 run = lrun[r];
     float acc[VE] = {};
     if (run.x < run.y) {
@@ -358,7 +369,7 @@ __global__ __launch_bounds__(ROW_THR) void k_row_grads(const T* __restrict__ g, 
 #pragma unroll
       for (int e = 0; e < VE; ++e) acc[e] *= scale;
     }
-    store_piece<T>(out + (v0 + r) * d + c0, acc, m, stream_out);
+    store_piece<T>(out + v * d + c0, acc, m, stream_out);
   }
 }
 
@@ -454,10 +465,15 @@ int launch_grad(const void* g, const Tokens& t, int d, float scale, void* out, c
   const int C = (d + VE - 1) / VE;
   // rows a workgroup: enough for its 256 threads, up to 2048 pieces while that leaves 2048 workgroups
   const int64_t want = std::min<int64_t>(2048, std::max<int64_t>(ROW_THR, V * C / 2048));
-  const int rows = std::min(MAX_ROWS, std::max(1, (int)(want / C)));
-  k_row_grads<T><<<(int)((V + rows - 1) / rows), ROW_THR, 0, st>>>((const T*)g, perm, w.runs, w.lv, V, d, w.dp, rows,
-                                                                  scale, V * d * (int64_t)sizeof(T) > STREAM_BYTES,
-                                                                  (T*)out);
+  const bool stream_out = V * d * (int64_t)sizeof(T) > STREAM_BYTES;
+  int grp = 0, lines = 0;  // at most 6: rows <= MAX_ROWS
+  while (C << grp < WAVE) ++grp;
+  while (((d * (int64_t)sizeof(T)) << lines) % 128) ++lines;
+  if (stream_out && (int64_t)C << lines <= 4096) grp = std::max(grp, lines);
+  const int rows = std::max(1, std::min(MAX_ROWS, (int)(want / C)) >> grp) << grp;
+  const int64_t dealt = (int64_t)DEAL * rows;
+  k_row_grads<T><<<(int)((V + dealt - 1) / dealt * DEAL), ROW_THR, 0, st>>>((const T*)g, perm, w.runs, w.lv, V, d, w.dp, rows,
+                                                                           grp, scale, stream_out, (T*)out);
   return check_launch("embedding gradient");
 }
 

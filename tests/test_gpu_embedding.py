@@ -109,6 +109,24 @@ def test_int32_shapes_strides_padding(V):
         assert torch.equal(grad, want)
 
 
+@pytest.mark.parametrize("V,d,dt", [(40000, 333, F16), (70001, 100, F32), (9001, 1024, F32), (131, 70000, F32), (5, 1000001, F32),
+                                    (3, 2000001, BF16), (600000, 7, F32), (4500000, 1, F32), (33, 64, BF16), (1000, 4, F32)])
+def test_every_row_is_written_once(V, d, dt):
+    """Outputs below and above the caches, rows that are whole 128-byte lines and rows that are not; small whole numbers,
+    so that each sum is exact in the type: at most 4 in absolute value, 255 / 4 of a row's tokens at the most."""
+    rng = np.random.default_rng(V + d)
+    n = 60 if d > 10000 else 3000
+    idx = torch.from_numpy(np.minimum(rng.zipf(1.3, n) - 1, V - 1))
+    idx[torch.bincount(idx, minlength=V)[idx] > 60] = -1  # rows that would pass 240 take nothing
+    g = torch.from_numpy(rng.integers(-4, 5, (n, d))).to(dt)
+    table = torch.empty(V, d, device=DEV, dtype=dt).requires_grad_(True)
+    out = A.embedding(table, idx.to(DEV))
+    got, = torch.autograd.grad(out, table, g.to(DEV))
+    want = torch.zeros(V, d)
+    want.index_add_(0, idx[idx >= 0], g[idx >= 0].float())
+    assert torch.equal(got.cpu().float(), want)
+
+
 @pytest.mark.parametrize("n", [100, 17000])
 def test_index_outside(n):
     """Rows that do not exist: a NaN output row, no gradient; the others are as without them."""
