@@ -11,7 +11,7 @@
 // numbers, x 2^E = hi + lo, hi and lo the roundings of x 2^E and of what is left (22 bits and a sign; 2^-37
 // in absolute terms for X), and
 //   P Q^T = hi hi^T + hi lo^T + lo hi^T      (lo lo^T is below 2^-24 of the product)
-// in one fp32 accumulator: three fp16 products at 8 times the fp32 matrix rate.  The matrix cores take
+// in one fp32 accumulator: three fp16 products, each at 16 times the fp32 matrix rate.  The matrix cores take
 // subnormal halves as they are.  E is 12 for X and A and 11 for B: the binding refuses coefficients whose
 // iteration leaves |s| <= 2 or |b s^2 + c s^4| <= 16, so nothing passes 2^15.
 //
