@@ -42,3 +42,13 @@ def test_c_entry_refuses():
     assert call(rows=0) == 0 and call(draws=0) == 0
     assert lib.regcn_sample(None, None) < 0
     assert lib.regcn_sample_workspace_bytes(0, 0, 0) >= 0
+
+
+@pytest.mark.parametrize("flag,value", [("--sample-draws", "-1"), ("--sample-temperature", "-0.5"), ("--sample-temperature", "inf"),
+                                        ("--sample-temperature", "nan"), ("--sample-top-k", "-2"), ("--sample-top-p", "1.5"),
+                                        ("--sample-top-p", "-0.1"), ("--sample-min-p", "2")])
+def test_the_command_refuses(flag, value):
+    """Before it loads anything."""
+    from regcn_amd import cli
+    with pytest.raises(ValueError, match="--sample"):
+        cli.main(["-d", "synthetic:icews14s_lgcn_roth", "--test", "--multi-step", "--sample-draws", "4", flag, value])
