@@ -332,6 +332,27 @@ class _Centroid(torch.autograd.Function):
         return dS0, dSv, None
 
 
+# ------------------------------------------------------------------- sums that replay
+SUM_STAGE = 4096
+
+
+def sum_last(x):
+    """x.sum(-1) in stages of SUM_STAGE elements.  torch sums many elements to one (131,072 and more measured) on
+    several workgroups and clears their tickets with a memset; in a replayed HIP graph such a sum returned
+    wrong values from the second replay on.  Up to 65,536 to one it stays in one workgroup."""
+    while x.shape[-1] > SUM_STAGE:
+        n = x.shape[-1]
+        whole = n // SUM_STAGE * SUM_STAGE
+        parts = x[..., :whole].unflatten(-1, (-1, SUM_STAGE)).sum(-1)
+        x = parts if whole == n else torch.cat([parts, x[..., whole:].sum(-1, keepdim=True)], -1)
+    return x.sum(-1)
+
+
+def total(x):
+    """x.sum(), as `sum_last`."""
+    return sum_last(x.reshape(-1))
+
+
 # ------------------------------------------------------------------------- cross entropy
 class _HypCE(torch.autograd.Function):
     """Per-query CE loss of the proxy score S = scale (margin - |(-q) (+) e|^2) + bias."""
@@ -369,13 +390,13 @@ class _HypCE(torch.autograd.Function):
         f = _lib.fptr
         _lib.call("regcn_hyp_ce_bwd_f32", f(q), f(cand), f(b) if ctx.has_bias else None, f(sc), f(mg),
                   _lib.iptr(tgt), f(lse), f(gl), B, N, d, ctx.c, 0, f(coef), f(rsum), f(csum), _lib.stream())
-        rs = rsum.sum(1, keepdim=True)
+        rs = sum_last(rsum).unsqueeze(1)
         cs = colsum(csum.reshape(ng, -1)).reshape(N, 3)
         dq = kreduce_mm(coef, cand, False, 2.0 * rs * q)            # coef E + 2 q sum_n G dS/d|q|^2
         de = kreduce_mm(coef, q, True, 2.0 * cs[:, :1] * cand)      # coef^T Q + 2 e sum_b G dS/d|e|^2
         dbias = cs[:, 1].clone() if ctx.has_bias else None
-        dscale = cs[:, 2].sum().reshape(ctx.scale_shape)
-        dmargin = (sc.reshape(()) * cs[:, 1].sum()).reshape(ctx.margin_shape)
+        dscale = total(cs[:, 2]).reshape(ctx.scale_shape)
+        dmargin = (sc.reshape(()) * total(cs[:, 1])).reshape(ctx.margin_shape)
         return dq, de, dbias, dscale, dmargin, None, None
 
 
@@ -440,18 +461,8 @@ def hyp_ce_loss(q, cand, target, c, bias=None, scale=None, margin=None, reductio
     return loss
 
 
-def _total(x):
-    """x.sum() in stages of 64 elements each.  torch's sum of many elements to one runs over several workgroups
-    and clears its tickets with a memset; in a replayed HIP graph such a sum returned wrong values from
-    the second replay on (the scale's and margin's gradients below).  Sums of 64 stay in one workgroup."""
-    x = x.reshape(-1)
-    while x.numel() > 64:
-        x = torch.nn.functional.pad(x, (0, -x.numel() % 64)).view(-1, 64).sum(1)
-    return x.sum()
-
-
 class _SpreadScalar(torch.autograd.Function):
-    """A 0-dim or one-element tensor over a shape; its gradient is the _total of the shape's."""
+    """A 0-dim or one-element tensor over a shape; its gradient is the total of the shape's."""
 
     @staticmethod
     def forward(ctx, s, shape):
@@ -460,7 +471,7 @@ class _SpreadScalar(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        return _total(g).reshape(ctx.shape), None
+        return total(g).reshape(ctx.shape), None
 
 
 def hyp_dist_ce_loss(q, cand, target, c_r, bias=None, scale=None, margin=None, reduction="mean"):

@@ -25,6 +25,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import analysis as _ana
+from .autograd import sum_last, total
 from .hyperbolic_decoder import (HyperbolicAttH, HyperbolicAttHRel, HyperbolicConvTransE, HyperbolicConvTransR,
                                  HyperbolicMuRP, HyperbolicMuRPRel, HyperbolicRotH, HyperbolicRotHRel,
                                  roth_pair_fusable, roth_pair_predict)
@@ -1106,11 +1107,11 @@ class HyperbolicRecurrentRGCN(nn.Module):
         if batch_size is None:
             seen = torch.zeros(self.num_ents, device=dev, dtype=torch.float32)
             seen.index_fill_(0, ents.reshape(-1), 1.0)
-            loss_radius = self.radius_lambda * (seen * diff * diff).sum() / seen.sum()
+            loss_radius = self.radius_lambda * total(seen * diff * diff) / total(seen)
         else:
             seen = torch.zeros(nb, self.num_ents, device=dev, dtype=torch.float32)
             seen.index_put_((seg.repeat_interleave(2), ents.reshape(-1)), torch.ones((), device=dev))
-            loss_radius = self.radius_lambda * (seen @ (diff * diff)) / seen.sum(1)
+            loss_radius = self.radius_lambda * (seen @ (diff * diff)) / sum_last(seen)
         return loss_ent, loss_rel, loss_static, loss_radius
 
     def log_gradient_stats(self):

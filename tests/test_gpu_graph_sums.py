@@ -1,0 +1,98 @@
+"""Sums of captured training steps against the same step run eagerly, on inputs that change between the replays (a
+sum whose workgroups' tickets are not cleared leaves its result of the replay before)."""
+import numpy as np
+import pytest
+import torch
+
+from regcn_amd import autograd as A
+from regcn_amd import cli
+from regcn_amd.weights import bump_versions
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+
+
+def replays_as_eager(step, leaves, times=4):
+    """step() -> tensors that follow from `leaves`: captured once and replayed, the leaves changed in place and eager
+    work done between the replays; every replay gives the eager bits."""
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = [o.detach() for o in step()]
+    for k in range(times):
+        with torch.no_grad():
+            for x in leaves:
+                x.mul_(1.0 + 0.01 * (k + 1))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = [o.detach().clone() for o in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.randn(300000, device=DEV).sum()
+        torch.cuda.synchronize()
+        for i, (o, w) in enumerate(zip(outs, want)):
+            assert torch.equal(o, w), "replay %d, output %d: off by %.3g of %.3g" % (
+                k, i, float((o - w).abs().max()), float(w.abs().max()))
+
+
+@pytest.mark.parametrize("n", [4097, 131072, 1000003])
+def test_totals(n):
+    x = torch.randn(n, 3, device=DEV)
+    replays_as_eager(lambda: [A.total(x), A.total(x[:, 1]), A.sum_last(x.t())], [x])
+
+
+@pytest.mark.parametrize("B,N", [(8, 200001), (300, 9000)])
+def test_cross_entropy_gradients(B, N):
+    g = torch.Generator().manual_seed(N)
+    q = (torch.randn(B, 16, generator=g) * 0.3).to(DEV).requires_grad_(True)
+    cand = (torch.randn(N, 16, generator=g) * 0.3).to(DEV).requires_grad_(True)
+    bias = torch.randn(N, generator=g).to(DEV).requires_grad_(True)
+    scale, margin = (torch.tensor(v, device=DEV).requires_grad_(True) for v in (1.5, 0.25))
+    target = torch.randint(0, N, (B,), generator=g).to(DEV)
+    leaves = [q, cand, bias, scale, margin]
+
+    def step():
+        loss = A.hyp_ce_loss(q, cand, target, 0.01, bias=bias, scale=scale, margin=margin)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    replays_as_eager(step, leaves)
+
+
+@pytest.mark.parametrize("batch", [None, 20])
+def test_step_with_many_entities(batch):
+    """140,000 entities: the losses and gradients of a whole step, its radius loss among them."""
+    V, R = 140000, 12
+    args = cli.build_parser().parse_args(
+        ["-d", "synthetic:icews14s_lgcn_roth", "--gpu", "0", "--encoder", "hyperbolic_uvrgcn", "--decoder", "roth",
+         "--n-hidden", "32", "--n-bases", "16", "--relation-prediction", "--entity-prediction", "--dropout", "0",
+         "--input-dropout", "0", "--hidden-dropout", "0", "--feat-dropout", "0"])
+    rng = np.random.default_rng(0)
+    snaps = [np.stack([rng.integers(0, V, 900), rng.integers(0, R, 900), rng.integers(0, V, 900)], 1) for _ in range(3)]
+    torch.manual_seed(0)
+    model = cli.build_model(args, V, R, snaps, DEV)
+    model.train()
+    graphs = cli.GraphCache(V, R, DEV)
+    glist = [graphs(s) for s in snaps[:2]]
+    triples = torch.from_numpy(snaps[2][:50].astype(np.int64)).to(DEV)
+    params = [p for p in model.parameters() if p.requires_grad]
+
+    def step():
+        for p in params:
+            p.grad = None
+        if batch is None:
+            losses = model.get_loss(glist, triples, None, True, query_time=2)
+            sum(l.sum() for l in losses).backward()
+        else:
+            parts = model.get_loss_batches(glist, triples, None, True, batch, query_time=2)
+            losses = [l for part in parts for l in part]
+        bump_versions(params)  # as after an optimizer step: caches made of the parameters are made again
+        return [l.detach() for l in losses] + [p.grad for p in params if p.grad is not None]
+    replays_as_eager(step, params)
