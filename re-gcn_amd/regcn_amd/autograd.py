@@ -27,6 +27,7 @@ the same per-pair scalars in float64 (hyp_dist_ce_loss).
 """
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -353,6 +354,55 @@ def total(x):
     return sum_last(x.reshape(-1))
 
 
+def sum_to(x, shape):
+    """x summed to a shape that broadcasts to its own, as `sum_last`.  Sums down columns go in stages of 64
+    rows: torch splits those earlier (3080 x 200 measured wrong in replays, 1025 x 64 not)."""
+    if math.prod(shape) == 1:
+        return total(x).reshape(shape)
+    x = x.contiguous()
+    lead = x.dim() - len(shape)
+    for k in range(x.dim()):
+        if x.shape[k] == 1 or k >= lead and shape[k - lead] != 1:
+            continue
+        if k == x.dim() - 1:
+            x = sum_last(x).unsqueeze(-1)
+            continue
+        while x.shape[k] > 64:
+            n = x.shape[k]
+            whole = n // 64 * 64
+            parts = x.narrow(k, 0, whole).unflatten(k, (-1, 64)).sum(k + 1)
+            x = parts if whole == n else torch.cat([parts, x.narrow(k, whole, n - whole).sum(k, keepdim=True)], k)
+        x = x.sum(k, keepdim=True)
+    return x.reshape(shape)
+
+
+class _Spread(torch.autograd.Function):
+    """t.expand(shape), whose gradient is `sum_to` t's shape."""
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(t, shape):
+        return t.expand(shape)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.small, ctx.shape = inputs[0].shape, inputs[1]
+
+    @staticmethod
+    def backward(ctx, g):
+        return sum_to(g, ctx.small), None
+
+    @staticmethod
+    def jvp(ctx, t, _):
+        return t.expand(ctx.shape)
+
+
+def spread(t, shape):
+    """t broadcast to a shape, for a parameter that many rows share: torch's own broadcasting, but the gradient's sum
+    replays in a HIP graph.  A Python number or None stays what it is."""
+    return _Spread.apply(t, torch.Size(shape)) if torch.is_tensor(t) else t
+
+
 # ------------------------------------------------------------------------- cross entropy
 class _HypCE(torch.autograd.Function):
     """Per-query CE loss of the proxy score S = scale (margin - |(-q) (+) e|^2) + bias."""
@@ -461,45 +511,31 @@ def hyp_ce_loss(q, cand, target, c, bias=None, scale=None, margin=None, reductio
     return loss
 
 
-class _SpreadScalar(torch.autograd.Function):
-    """A 0-dim or one-element tensor over a shape; its gradient is the total of the shape's."""
-
-    @staticmethod
-    def forward(ctx, s, shape):
-        ctx.shape = s.shape
-        return s.detach().reshape(()).expand(shape).clone()
-
-    @staticmethod
-    def backward(ctx, g):
-        return total(g).reshape(ctx.shape), None
-
-
 def hyp_dist_ce_loss(q, cand, target, c_r, bias=None, scale=None, margin=None, reduction="mean"):
     """mean CE of the arctanh-distance score with per-query curvatures c_r
     (hyperbolic_decoder.py:257-283): logits = scale (margin - d_{c_r}(q, e)) + bias,
     d = 2 / (sqrt(c_r + eps) + eps) atanh(min(sqrt(c_r + eps) min(|n| / (den + eps), bound),
     1 - eps)).  Per-pair scalars in float64, autograd through q, e, c_r, bias, scale, margin."""
     qd, ed = q.double(), cand.double()
+    wide = lambda t: spread(t.double() if torch.is_tensor(t) else t, (q.shape[0], cand.shape[0]))  # noqa: E731
     c = c_r.double().reshape(-1, 1)
     sqrt_c = torch.sqrt(c + EPS)
     x2 = (qd * qd).sum(1, keepdim=True)
-    y2 = (ed * ed).sum(1).unsqueeze(0)
+    y2 = wide((ed * ed).sum(1).unsqueeze(0))
     xy = qd @ ed.t()
-    A = 1 - 2 * c * xy + c * y2  # num = A (-q) + B e
+    cxy = wide(2 * c) * xy
+    A = 1 - cxy + wide(c) * y2  # num = A (-q) + B e
     Bc = 1 - c * x2
-    num2 = A * A * x2 - 2 * A * Bc * xy + Bc * Bc * y2
-    den = 1 - 2 * c * xy + c * c * x2 * y2
+    num2 = A * A * wide(x2) - 2 * A * wide(Bc) * xy + wide(Bc * Bc) * y2
+    den = 1 - cxy + wide(c * c * x2) * y2
     n = (num2.clamp(min=1e-30).sqrt() / (den + EPS).abs()).clamp(min=EPS)
-    n = torch.min(n, 1.0 / (sqrt_c + EPS) - EPS)
-    dist = (2.0 / (sqrt_c + EPS)) * torch.atanh((sqrt_c * n).clamp(max=1.0 - EPS))
-    if torch.is_tensor(margin):
-        logits = _SpreadScalar.apply(margin.double(), dist.shape) - dist
-    else:
-        logits = (0.0 if margin is None else margin) - dist
+    n = torch.min(n, wide(1.0 / (sqrt_c + EPS) - EPS))
+    dist = wide(2.0 / (sqrt_c + EPS)) * torch.atanh((wide(sqrt_c) * n).clamp(max=1.0 - EPS))
+    logits = (0.0 if margin is None else wide(margin)) - dist
     if scale is not None:
-        logits = (_SpreadScalar.apply(scale.double(), dist.shape) if torch.is_tensor(scale) else scale) * logits
+        logits = wide(scale) * logits
     if bias is not None:
-        logits = logits + bias.double()
+        logits = logits + wide(bias)
     return torch.nn.functional.cross_entropy(logits, target.long(), reduction=reduction).float()
 
 
