@@ -614,6 +614,31 @@ def linear(layer, x):
     return layer(x)
 
 
+class _GruGates(torch.autograd.Function):
+    """A GRU cell's gates and new state from its two products; the bias gradients on `colsum`."""
+
+    @staticmethod
+    def forward(ctx, gi, gh, h, b_ih, b_hh):
+        out, ws = torch.ops.aten._thnn_fused_gru_cell(gi, gh, h, b_ih, b_hh)
+        ctx.save_for_backward(ws)
+        return out
+
+    @staticmethod
+    def backward(ctx, gy):
+        di, dh, dx = torch.ops.aten._thnn_fused_gru_cell_backward(gy.contiguous(), ctx.saved_tensors[0], False)[:3]
+        need = ctx.needs_input_grad
+        return di, dh, dx, colsum(di) if need[3] else None, colsum(dh) if need[4] else None
+
+
+def gru_cell(cell, x, h):
+    """cell(x, h) for an nn.GRUCell (the relation GRU, hyperbolic_model.py:815-823): torch's products and fused gates.
+    With gradients its biases' sums over the rows (2R x 3d) are those of `colsum`."""
+    if x.is_cuda and x.dim() == 2 and x.dtype == torch.float32 and cell.bias and needs_grad(x, h, *cell.parameters()):
+        return _GruGates.apply(torch.mm(x, cell.weight_ih.t()), torch.mm(h, cell.weight_hh.t()), h.contiguous(), cell.bias_ih,
+                               cell.bias_hh)
+    return cell(x, h)
+
+
 class _RowsByWeight(torch.autograd.Function):
     """x (V x d_in) @ W (d_in x d_out): forward and the input gradient dy W^T are library GEMMs
     (large M, short K); the weight gradient x^T dy (K = V) runs on regcn_kreduce_gemm_f32."""

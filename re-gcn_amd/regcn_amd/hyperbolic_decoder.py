@@ -129,7 +129,7 @@ def givens_rotation(x, angles):
         if fused is not None:
             return fused
     if angles.dim() == 1:
-        angles = angles.unsqueeze(0).expand(x.shape[0], -1)
+        angles = _ag.spread(angles, (x.shape[0], angles.shape[0]))
     x1, x2 = x[:, 0::2], x[:, 1::2]
     co, si = torch.cos(angles), torch.sin(angles)
     return torch.stack([co * x1 - si * x2, si * x1 + co * x2], dim=2).reshape(x.shape[0], x.shape[1])
@@ -142,7 +142,7 @@ def givens_reflection(x, angles):
         if fused is not None:
             return fused
     if angles.dim() == 1:
-        angles = angles.unsqueeze(0).expand(x.shape[0], -1)
+        angles = _ag.spread(angles, (x.shape[0], angles.shape[0]))
     x1, x2 = x[:, 0::2], x[:, 1::2]
     co, si = torch.cos(angles), torch.sin(angles)
     return torch.stack([co * x1 + si * x2, si * x1 - co * x2], dim=2).reshape(x.shape[0], x.shape[1])
@@ -589,7 +589,8 @@ class HyperbolicConvTransE(nn.Module):
         x = self.hidden_drop(_ag.linear(self.fc, x.view(B, -1)))
         if B > 1:
             x = _ag.batch_norm(self.bn2, x)
-        return torch.mm(F.relu(x), et.transpose(1, 0)) + self.b
+        scores = torch.mm(F.relu(x), et.transpose(1, 0))
+        return scores + _ag.spread(self.b, scores.shape)
 
 
 class HyperbolicConvTransR(nn.Module):
@@ -618,4 +619,5 @@ class HyperbolicConvTransR(nn.Module):
         x = torch.cat([_take(self, et, triplets[:, 0]).unsqueeze(1), _take(self, et, triplets[:, 2]).unsqueeze(1)], 1)
         x = self.feature_map_drop(F.relu(_ag.batch_norm(self.bn1, self.conv1(self.inp_drop(_ag.batch_norm(self.bn0, x))))))
         x = _ag.batch_norm(self.bn2, self.hidden_drop(_ag.linear(self.fc, x.view(B, -1))))
-        return torch.mm(F.relu(x), rel_embedding.transpose(1, 0)) + self.b
+        scores = torch.mm(F.relu(x), rel_embedding.transpose(1, 0))
+        return scores + _ag.spread(self.b, scores.shape)

@@ -153,7 +153,7 @@ def relation_context(x, g, R2):
     """x_input[r] = mean of the rows of r's r_to_e span, 0 for absent relations
     (hyperbolic_model.py:802-812), HIP forward and backward (_RelationContext)."""
     if g.work()["rel_idx"].numel() == 0:
-        return torch.zeros(R2, x.shape[1], device=x.device, dtype=x.dtype) + 0.0 * x.sum()
+        return torch.zeros(R2, x.shape[1], device=x.device, dtype=x.dtype) + x[:0].sum()
     return _RelationContext.apply(x, g, R2)
 
 
@@ -180,7 +180,7 @@ def model_forward(model, g_list):
         g = g.to(dev)
         x_prev = A.log0(h, ct)                                                         # :802
         x_in = torch.cat([model.emb_rel, relation_context(x_prev, g, R2)], dim=1)
-        h0 = model.relation_gru(x_in, model.emb_rel if i == 0 else h0)                 # :815-823
+        h0 = A.gru_cell(model.relation_gru, x_in, model.emb_rel if i == 0 else h0)     # :815-823
         if model.layer_norm:
             h0 = F.normalize(h0)
         cur = cell_forward(model.rgcn, g, h, [h0] * len(model.rgcn.layers), lorentz)   # :828
@@ -238,7 +238,7 @@ def euclid_model_forward(model, g_list):
     for i, g in enumerate(g_list):
         g = g.to(dev)
         x_in = torch.cat([model.emb_rel, relation_context(h, g, R2)], dim=1)
-        h0 = model.relation_cell_1(x_in, model.emb_rel if i == 0 else h0)
+        h0 = A.gru_cell(model.relation_cell_1, x_in, model.emb_rel if i == 0 else h0)
         if model.layer_norm:
             h0 = F.normalize(h0)
         cur = h

@@ -6,6 +6,7 @@ import torch
 
 from regcn_amd import autograd as A
 from regcn_amd import cli
+from regcn_amd import hyperbolic_decoder as D
 from regcn_amd.weights import bump_versions
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,59 @@ def test_step_with_many_entities(batch):
         bump_versions(params)  # as after an optimizer step: caches made of the parameters are made again
         return [l.detach() for l in losses] + [p.grad for p in params if p.grad is not None]
     replays_as_eager(step, params)
+
+
+@pytest.mark.parametrize("rows", [7, 460, 512, 3000])
+def test_gru_cell(rows):
+    """torch's own cell to the bit but for the order of the bias gradients' sums: at most `rows` additions of fp32 terms,
+    rows 2^-24 of the sum of their magnitudes."""
+    torch.manual_seed(rows)
+    cell = torch.nn.GRUCell(80, 40).to(DEV)
+    x, h = (torch.randn(rows, n, device=DEV).requires_grad_(True) for n in (80, 40))
+    g = torch.randn(rows, 40, device=DEV)
+    leaves = [x, h, *cell.parameters()]
+    out = A.gru_cell(cell, x, h)
+    want = cell(x, h)
+    assert torch.equal(out, want)
+    got, ref = torch.autograd.grad(out, leaves, g), torch.autograd.grad(want, leaves, g)
+    for (name, _), a, b in zip([("x", 0), ("h", 0), *cell.named_parameters()], got, ref):
+        if name.startswith("bias"):  # |g| <= 6 and a gate's factors are below 1
+            assert float((a - b).abs().max()) <= 2 * rows * 2.0 ** -24 * rows * 6.0
+        else:
+            assert torch.equal(a, b), name
+    del out, want
+    replays_as_eager(lambda: [*torch.autograd.grad(A.gru_cell(cell, x, h), leaves, g)], leaves + [g])
+
+
+@pytest.mark.parametrize("B", [64, 3080])
+@pytest.mark.parametrize("turn", [D.givens_rotation, D.givens_reflection])
+def test_angles_that_all_rows_share(B, turn):
+    x, angles = torch.randn(B, 200, device=DEV).requires_grad_(True), torch.randn(100, device=DEV).requires_grad_(True)
+    g = torch.randn(B, 200, device=DEV)
+    replays_as_eager(lambda: [*torch.autograd.grad(turn(x, angles), [x, angles], g)], [x, angles, g])
+    rows = angles.detach().expand(B, 100).contiguous()
+    assert torch.equal(turn(x.detach(), angles.detach()), turn(x.detach(), rows))
+
+
+@pytest.mark.parametrize("B,N", [(3080, 460), (70, 9000)])
+def test_distance_cross_entropy_gradients(B, N):
+    g = torch.Generator().manual_seed(B)
+    q, cand = ((torch.randn(n, 8, generator=g) * 0.3).to(DEV).requires_grad_(True) for n in (B, N))
+    c, bias = ((torch.rand(n, generator=g) + 0.05).to(DEV).requires_grad_(True) for n in (B, N))
+    scale, margin = (torch.tensor(v, device=DEV).requires_grad_(True) for v in (1.5, 0.25))
+    target = torch.randint(0, N, (B,), generator=g).to(DEV)
+    leaves = [q, cand, c, bias, scale, margin]
+
+    def step():
+        loss = A.hyp_dist_ce_loss(q, cand, target, c, bias=bias, scale=scale, margin=margin)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    replays_as_eager(step, leaves)
+
+
+def test_convolutional_relation_scores_bias():
+    torch.manual_seed(0)
+    dec = D.HyperbolicConvTransR(256, 40).to(DEV)
+    ent, rel = torch.randn(50, 40, device=DEV) * 0.1, torch.randn(512, 40, device=DEV) * 0.1
+    tri = torch.randint(0, 50, (3080, 3), device=DEV)
+    g = torch.randn(3080, 512, device=DEV)
+    replays_as_eager(lambda: [*torch.autograd.grad(dec(ent, rel, tri), [dec.b], g)], [g])
