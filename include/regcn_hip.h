@@ -841,6 +841,11 @@ int regcn_hyp_ce_bwd_f32(const float* q, const float* cand, const float* bias, c
                          int32_t B, int32_t N, int32_t d, float c, int32_t flags, float* coef, float* rsum,
                          float* csum, void* stream);
 
+/* ---- Captured graphs ------------------------------------------------------------------------ */
+/* The memset nodes of a captured hipGraph_t into *count.  Such nodes have not cleared their memory in replays after
+ * the first one; a graph that holds some (library reductions over several workgroups record them) must not be replayed. */
+int regcn_graph_memset_nodes(void* graph, int64_t* count);
+
 /* ---- Embedding rows ------------------------------------------------------------------- */
 /* out[i, :] = scale * table[idx[i], :], one rounding to `dtype`.  table: V rows of d elements,
  * `ld` elements apart (any element-aligned address); idx: n int32 (idx_wide = 0) or int64 indices;

@@ -1,6 +1,7 @@
 // extern "C" entry points of libregcn_hip.so (declared in include/regcn_hip.h).
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include "regcn_internal.h"
 
@@ -781,6 +782,24 @@ int regcn_snapshot_row_type_order_i32(int32_t V, int32_t E, int32_t R2, const in
                                       const int32_t* col_type, int32_t* out_src, int32_t* out_type, void* workspace,
                                       size_t ws_bytes, void* s) {
   return row_type_order(V, E, R2, rowptr, col_src, col_type, out_src, out_type, workspace, ws_bytes, ST(s));
+}
+
+int regcn_graph_memset_nodes(void* graph, int64_t* count) {
+  if (!graph || !count) return set_error(REGCN_EINVAL, "graph_memset_nodes: null graph or count");
+  size_t n = 0;
+  hipError_t rc = hipGraphGetNodes((hipGraph_t)graph, nullptr, &n);
+  hipGraphNode_t* nodes = n ? (hipGraphNode_t*)malloc(n * sizeof(hipGraphNode_t)) : nullptr;
+  if (n && !nodes) return set_error(REGCN_EINVAL, "graph_memset_nodes: no host memory for %zu nodes", n);
+  if (rc == hipSuccess && n) rc = hipGraphGetNodes((hipGraph_t)graph, nodes, &n);
+  *count = 0;
+  for (size_t i = 0; rc == hipSuccess && i < n; ++i) {
+    hipGraphNodeType type;
+    rc = hipGraphNodeGetType(nodes[i], &type);
+    if (rc == hipSuccess && type == hipGraphNodeTypeMemset) ++*count;
+  }
+  free(nodes);
+  if (rc != hipSuccess) return set_error((int)rc, "graph_memset_nodes: %s", hipGetErrorString(rc));
+  return 0;
 }
 
 int regcn_embedding(const void* table, int64_t ld, const void* idx, int32_t idx_wide, int64_t n, int64_t V, int32_t d,

@@ -105,6 +105,7 @@ _SIGS = {
     "regcn_lorentz_aggregate_bwd_f32": [P, _c_int, _c_f, P],
     "regcn_hyp_ce_lse_f32": [P, P, P, P, P, P, _c_int, _c_int, _c_int, _c_f, _c_int, P, P, P, P],
     "regcn_hyp_ce_bwd_f32": [P, P, P, P, P, P, P, P, _c_int, _c_int, _c_int, _c_f, _c_int, P, P, P, P],
+    "regcn_graph_memset_nodes": [P, P],
     "regcn_embedding": [P, _c_i64, P, _c_int, _c_i64, _c_i64, _c_int, _c_int, _c_f, P, P],
     "regcn_embedding_grad_workspace_bytes": [_c_i64, _c_i64, _c_int],
     "regcn_embedding_grad": [P, P, _c_int, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_f, P, P, _c_sz, P],
@@ -300,6 +301,13 @@ def call(name, *args):
 def call_layer(desc):
     check(lib().regcn_layer_f32(ctypes.byref(desc), stream()),
           "regcn_layer_f32(step)" if desc.fuse_step else "regcn_layer_f32")
+
+
+def graph_memset_nodes(graph):
+    """Memset nodes of a torch.cuda.CUDAGraph captured with keep_graph=True (regcn_graph_memset_nodes)."""
+    n = _c_i64()
+    check(lib().regcn_graph_memset_nodes(graph.raw_cuda_graph(), ctypes.byref(n)), "regcn_graph_memset_nodes")
+    return n.value
 
 
 def publish():

@@ -12,12 +12,16 @@ normalize, GRUCell) as device torch ops.  The op sequence is the reference's:
   LorentzRGCNLayer.forward           hyperbolic_layers.py:627-694
   HyperbolicRecurrentRGCN.forward    hyperbolic_model.py:722-890
 """
+import logging
+
 import torch
 import torch.nn.functional as F
 
 from . import _lib
 from . import analysis
 from . import autograd as A
+
+logger = logging.getLogger("regcn_amd.training")
 
 RRELU_SLOPE = (1.0 / 8 + 1.0 / 3) / 2  # F.rrelu(x) with training=False (hyperbolic_model.py:120)
 
@@ -273,7 +277,10 @@ class GraphedSteps:
     sample's snapshot graphs and triples, which the caller keeps alive for the key, and
     writes parameters, optimizer state and its returned tensor), so replays may come in any
     order; the returned tensor is valid until the next `run`.  Dropout draws from the
-    graph-safe generator (a different mask per replay, as in eager steps)."""
+    graph-safe generator (a different mask per replay, as in eager steps).
+
+    A step whose capture holds memset nodes is not replayed, since those do not clear their memory in later replays
+    (torch's sums over several workgroups record them): it runs eagerly each time, with one warning."""
 
     def __init__(self, device):
         self.device = device
@@ -289,14 +296,21 @@ class GraphedSteps:
         self.stream.wait_stream(cur)
         with torch.cuda.stream(self.stream):
             g = self.graphs.get(key)
-            if g is not None:
+            if g is not None and g[0] is not None:
                 g[0].replay()
                 out = g[1]
             else:
                 out = step()  # eager: lazily built caches (transposed edge lists, ...) exist after it
-                gph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(gph, pool=self.pool, stream=self.stream):
-                    static = step()
-                self.graphs[key] = (gph, static)
+                if g is None:
+                    gph = torch.cuda.CUDAGraph(keep_graph=True)
+                    with torch.cuda.graph(gph, pool=self.pool, stream=self.stream):
+                        static = step()
+                    memsets = _lib.graph_memset_nodes(gph)
+                    if memsets:
+                        logger.warning("step %r runs eagerly: its graph holds %d memset nodes", key, memsets)
+                        self.graphs[key] = (None, None)
+                    else:
+                        gph.instantiate()
+                        self.graphs[key] = (gph, static)
         cur.wait_stream(self.stream)
         return out

@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 import torch
 
+from regcn_amd import _lib
 from regcn_amd import autograd as A
-from regcn_amd import cli
+from regcn_amd import cli, muon, ranking, training
 from regcn_amd import hyperbolic_decoder as D
 from regcn_amd.weights import bump_versions
 
@@ -153,3 +154,58 @@ def test_convolutional_relation_scores_bias():
     tri = torch.randint(0, 50, (3080, 3), device=DEV)
     g = torch.randn(3080, 512, device=DEV)
     replays_as_eager(lambda: [*torch.autograd.grad(dec(ent, rel, tri), [dec.b], g)], [g])
+
+
+def test_steps_whose_graph_would_not_replay_run_eagerly(caplog):
+    """A sum over several workgroups in a step: right on every run, where a replay would not be; the other keys replay."""
+    x = torch.ones(1 << 20, device=DEV)
+    steps, calls = training.GraphedSteps(DEV), {"sum": 0, "total": 0}
+
+    def step(name):
+        calls[name] += 1
+        return x.sum() if name == "sum" else A.total(x)
+    for k in range(1, 5):
+        x.fill_(float(k))
+        for name in calls:
+            assert float(steps.run(name, lambda: step(name))) == float(k << 20)
+    assert calls == {"sum": 5, "total": 2}  # the capture's own call among them
+    assert sum("memset" in r.message for r in caplog.records) == 1
+
+
+@pytest.mark.parametrize("encoder,decoder,extra", [
+    ("lgcn", "roth", []), ("hyperbolic_uvrgcn", "roth", ["--no-reuse-encoder"]), ("hyperbolic_uvrgcn", "atth", []),
+    ("hyperbolic_uvrgcn", "murp", ["--sorted-lookup"]), ("hyperbolic_uvrgcn", "hyperbolic_convtranse", []),
+    ("lgcn", "roth", ["--plus-relation-specific-curvature"])])
+def test_training_steps_hold_no_memset_nodes(encoder, decoder, extra):
+    """Whole steps of 3,080 queries over 23,033 entities and 512 relations, both optimisers among them: --hip-graph
+    replays them."""
+    args = cli.build_parser().parse_args(
+        ["-d", "synthetic:icews18_roth", "--gpu", "0", "--encoder", encoder, "--decoder", decoder, "--n-hidden", "200",
+         "--synthetic-snapshots", "5", "--relation-prediction", "--entity-prediction", "--optimizer", "muon", *extra])
+    torch.manual_seed(0)
+    V, R, train, _, _ = cli.load_dataset(args)
+    tl = ranking.split_by_time(train)
+    model = training.use_sorted_lookup(cli.build_model(args, V, R, tl, DEV), args.sorted_lookup)
+    model.train()
+    graphs = cli.GraphCache(V, R, DEV)
+    glist = [graphs(s) for s in tl[:2]]
+    triples = torch.from_numpy(np.asarray(tl[2], dtype=np.int64)).to(DEV)
+    mats, rest = muon.split_parameters(model)
+    optimizer = cli.Optimizers(muon.Muon(mats), torch.optim.Adam(rest, capturable=True, fused=True))
+
+    def step():
+        optimizer.zero_grad()
+        if args.reuse_encoder:
+            model.get_loss_batches(glist, triples, None, True, args.triple_batch_size, query_time=2)
+        else:
+            sum(l.sum() for l in model.get_loss(glist, triples, None, True, query_time=2)).backward()
+        torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
+        optimizer.step()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    assert _lib.graph_memset_nodes(graph) == 0

@@ -1,7 +1,10 @@
 """The staged sums of autograd.py: whole numbers, so every order of summation is exact."""
+import ctypes
+
 import pytest
 import torch
 
+from regcn_amd import _lib
 from regcn_amd import autograd as A
 
 S = A.SUM_STAGE
@@ -93,3 +96,10 @@ def test_forward_mode_through_scale_and_margin():
     s, m = scale.clone().requires_grad_(True), margin.clone().requires_grad_(True)
     ds, dm = torch.autograd.grad(f(s, m), (s, m))
     assert abs(float(tangent) - float(ds + 2 * dm)) <= 2.0 ** -24 * abs(float(ds + 2 * dm)) + 1e-10
+
+
+def test_graph_entry_refuses():
+    n = ctypes.c_int64(7)
+    assert _lib.lib().regcn_graph_memset_nodes(None, ctypes.byref(n)) < 0
+    assert _lib.lib().regcn_graph_memset_nodes(ctypes.byref(n), None) < 0
+    assert b"graph_memset_nodes" in _lib.lib().regcn_last_error_string()
