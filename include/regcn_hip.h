@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define REGCN_ABI_VERSION 13
+#define REGCN_ABI_VERSION 14
 #define REGCN_EINVAL (-1)
 #define REGCN_ENOTSUP (-2)
 
@@ -886,14 +886,15 @@ typedef struct regcn_sample_desc {
   int32_t top_k;                  /* <= 0 or >= cols: off */
   double temperature;             /* not above 0: the first of the order */
   double top_p, min_p;            /* >= 1: off; <= 0: off */
-  const float* temperature_rows;  /* one per row in place of the number above, or NULL */
+  const void* temperature_rows;   /* one float or double per row in place of the number above, or NULL */
   const int32_t* top_k_rows;
-  const float* top_p_rows;
-  const float* min_p_rows;
+  const void* top_p_rows;
+  const void* min_p_rows;
   int64_t* ids;                   /* rows x draws: the drawn column, -1 for a row without a score to take */
   float* logp;                    /* rows x draws: log of the draw's probability (-inf with -1), or NULL */
   void* workspace;                /* regcn_sample_workspace_bytes (0: may be NULL) */
   size_t ws_bytes;
+  int32_t rows_wide;              /* 1: temperature_rows holds doubles; 2: top_p_rows; 4: min_p_rows */
 } regcn_sample_desc;
 /* Per row: weights exp((s - max) / temperature); kept are, in the order "larger score first, ties by lower
  * column", the first top_k, of those the shortest prefix whose weights reach top_p of their sum, and of those

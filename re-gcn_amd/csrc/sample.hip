@@ -52,8 +52,9 @@ struct RowArgs {
   const void* u;
   double temperature, top_p, min_p;
   int32_t top_k, shift;  // shift: S
-  const float *temperature_v, *top_p_v, *min_p_v;
+  const void *temperature_v, *top_p_v, *min_p_v;
   const int32_t* top_k_v;
+  int32_t rows_wide;  // which of the three are doubles: bits 0, 1, 2
   int64_t* ids;
   float* logp;
   ExpConsts c;
@@ -68,12 +69,16 @@ struct Limits {
   bool ties_only;  // an infinite score, or a temperature whose inverse is: weight only on the largest
 };
 
+__device__ __forceinline__ double row_value(const void* v, int wide, int row, double all) {
+  return !v ? all : wide ? ((const double*)v)[row] : (double)((const float*)v)[row];
+}
+
 __device__ __forceinline__ Limits row_limits(const RowArgs& a, int row) {
   Limits l;
-  const double t = a.temperature_v ? (double)a.temperature_v[row] : a.temperature;
+  const double t = row_value(a.temperature_v, a.rows_wide & 1, row, a.temperature);
   const int k = a.top_k_v ? a.top_k_v[row] : a.top_k;
-  const double m = a.min_p_v ? (double)a.min_p_v[row] : a.min_p;
-  l.top_p = a.top_p_v ? (double)a.top_p_v[row] : a.top_p;
+  const double m = row_value(a.min_p_v, a.rows_wide & 4, row, a.min_p);
+  l.top_p = row_value(a.top_p_v, a.rows_wide & 2, row, a.top_p);
   l.min_w = m > 0 ? __builtin_ldexp(m < 1.0 ? m : 1.0, a.shift) : 0.0;
   l.top_k = k > 0 && k < a.cols ? (uint32_t)k : ALL;
   l.inv_t = 1.0 / t;
@@ -966,6 +971,7 @@ int dispatch(const RowArgs& a, void* ws, hipStream_t st) {
   if (a.cols <= 24576) return launch<T, 1024, 24576>(a, st);
   if (a.cols <= ROW_MAX) return launch<T, 1024, ROW_MAX>(a, st);
   RowArgs part = a;
+  const auto from = [&](const void* v, int wide, int64_t r0) { return v ? (const char*)v + r0 * (wide ? 8 : 4) : nullptr; };
   const int most = rows_at_once(a.cols);
   for (int r0 = 0; r0 < a.rows; r0 += most) {
     part.rows = std::min(most, a.rows - r0);
@@ -973,10 +979,10 @@ int dispatch(const RowArgs& a, void* ws, hipStream_t st) {
     part.u = (const char*)a.u + (int64_t)r0 * a.draws * (a.u_wide ? 8 : 4);
     part.ids = a.ids + (int64_t)r0 * a.draws;
     part.logp = a.logp ? a.logp + (int64_t)r0 * a.draws : nullptr;
-    part.temperature_v = a.temperature_v ? a.temperature_v + r0 : nullptr;
+    part.temperature_v = from(a.temperature_v, a.rows_wide & 1, r0);
     part.top_k_v = a.top_k_v ? a.top_k_v + r0 : nullptr;
-    part.top_p_v = a.top_p_v ? a.top_p_v + r0 : nullptr;
-    part.min_p_v = a.min_p_v ? a.min_p_v + r0 : nullptr;
+    part.top_p_v = from(a.top_p_v, a.rows_wide & 2, r0);
+    part.min_p_v = from(a.min_p_v, a.rows_wide & 4, r0);
     if (int rc = launch_spread<T>(part, ws, st)) return rc;
   }
   return 0;
@@ -1016,6 +1022,7 @@ int sample(const regcn_sample_desc& d, hipStream_t st) {
   a.top_k_v = d.top_k_rows;
   a.top_p_v = d.top_p_rows;
   a.min_p_v = d.min_p_rows;
+  a.rows_wide = d.rows_wide;
   a.ids = d.ids;
   a.logp = d.logp;
   a.c.log2e = 1.4426950408889634074;

@@ -15,7 +15,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("REGCN_HIP_LIB") or os.path.join(_HERE, "libregcn_hip.so")  # override: A/B builds
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _c_int, _c_i64, _c_f, _c_vp, _c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 P = _c_vp
@@ -214,7 +214,8 @@ class SampleDesc(ctypes.Structure):
     _fields_ = [("score", P), ("ld", _c_i64), ("rows", _c_int), ("cols", _c_int), ("draws", _c_int), ("dtype", _c_int),
                 ("u", P), ("u_wide", _c_int), ("top_k", _c_int), ("temperature", ctypes.c_double),
                 ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("temperature_rows", P), ("top_k_rows", P),
-                ("top_p_rows", P), ("min_p_rows", P), ("ids", P), ("logp", P), ("workspace", P), ("ws_bytes", _c_sz)]
+                ("top_p_rows", P), ("min_p_rows", P), ("ids", P), ("logp", P), ("workspace", P), ("ws_bytes", _c_sz),
+                ("rows_wide", _c_int)]
 
 
 class SnapshotDesc(ctypes.Structure):

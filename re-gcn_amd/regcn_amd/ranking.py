@@ -90,13 +90,28 @@ def get_total_rank(test_triples, score, all_ans, eval_bz, rel_predict=0):
 _SAMPLE_MAX_COLS = 1 << 24
 
 
-def _limit(value, name, rows, device, dtype, low, high, high_in=True):
+def _row_limits(value, whole):
+    """A limit's values per row as the kernel reads them, none narrowed: whole numbers clamped to int32, others in fp32
+    where that holds their type, else fp64."""
+    if whole:
+        if value.is_floating_point():
+            value = value.nan_to_num(0.0).clamp(0.0, 2.0 ** 30)
+        if value.dtype != torch.int32:
+            value = value.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)
+    elif value.dtype in (torch.bfloat16, torch.float16):
+        value = value.float()
+    elif value.dtype != torch.float32:
+        value = value.double()
+    return value.contiguous()
+
+
+def _limit(value, name, rows, device, whole, low, high, high_in=True):
     """(number, device tensor of one per row or None) of a sampling limit."""
     if isinstance(value, torch.Tensor) and value.dim() > 0:
         if value.shape != (rows,) or value.device != device:
             raise ValueError("%s must be one number or a tensor of %d on %s (got %s on %s)"
                              % (name, rows, device, tuple(value.shape), value.device))
-        return 0, value.to(dtype).contiguous()
+        return 0, _row_limits(value, whole)
     v = float(value)
     if not (low <= v < high or high_in and v == high):
         raise ValueError("%s must lie between %g and %g (got %r)" % (name, low, high, value))
@@ -132,10 +147,10 @@ def sample(score, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp
     if cols > _SAMPLE_MAX_COLS:
         raise ValueError("rows of up to %d scores (got %d)" % (_SAMPLE_MAX_COLS, cols))
     dev = score.device
-    t, t_rows = _limit(temperature, "temperature", rows, dev, torch.float32, 0.0, float("inf"), False)
-    k, k_rows = _limit(top_k, "top_k", rows, dev, torch.int32, 0, 2 ** 31 - 1)
-    p, p_rows = _limit(top_p, "top_p", rows, dev, torch.float32, 0.0, 1.0)
-    m, m_rows = _limit(min_p, "min_p", rows, dev, torch.float32, 0.0, 1.0)
+    t, t_rows = _limit(temperature, "temperature", rows, dev, False, 0.0, float("inf"), False)
+    k, k_rows = _limit(top_k, "top_k", rows, dev, True, 0, 2 ** 31 - 1)
+    p, p_rows = _limit(top_p, "top_p", rows, dev, False, 0.0, 1.0)
+    m, m_rows = _limit(min_p, "min_p", rows, dev, False, 0.0, 1.0)
     if not score.is_cuda or u.device != dev:
         raise ValueError("score and u must live on one HIP device (got %s, %s); the HIP path has no CPU fallback"
                          % (dev, u.device))
@@ -158,6 +173,7 @@ def sample(score, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp
                         ("min_p_rows", m_rows), ("logp", logp)):
             if v is not None:
                 setattr(d, name, v.data_ptr())
+        d.rows_wide = sum(b for b, v in ((1, t_rows), (2, p_rows), (4, m_rows)) if v is not None and v.dtype == torch.float64)
         d.ws_bytes = _lib.lib().regcn_sample_workspace_bytes(rows, cols, d.dtype)
         if d.ws_bytes:
             ws = torch.empty(d.ws_bytes, device=dev, dtype=torch.uint8)

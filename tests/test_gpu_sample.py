@@ -250,3 +250,23 @@ def test_large_offsets():
     u = torch.full((2200,), 0.5, dtype=torch.float64, device=DEV)
     got = ranking.sample(s, u, top_k=1)
     assert int(got[2199]) == 77777 and int(got[2100]) == 1000002 and int(got[0]) == 0
+
+
+@pytest.mark.parametrize("N", [40, 5000, 40000])
+def test_limits_per_row_in_64_bits(N):
+    """A limit given per row keeps what the same number keeps for all rows, its bits beyond fp32 and int32 among them.
+    The weights are 1, 1/2, 1/4, ...: top_p = 3/4 of a sum of 2 - 2^-39 keeps two, a little less one more or fewer."""
+    s, u = make(6, N, 5, 21)
+    s[0] = -float("inf")
+    s[0, :40] = -math.log(2.0) * torch.arange(40, dtype=torch.float64).float().to(DEV)
+    s[1:3] = s[0]
+    full = lambda v, dt=torch.float64: torch.full((6,), v, dtype=dt, device=DEV)  # noqa: E731
+    for T in (1.0, 0.7, 1.0 / 3.0):
+        for p in (0.9, 0.75, 0.75 - 1e-12, 0.75 + 1e-9, 1.0 / 3.0):
+            for m in (0.0, 0.1, 0.25):
+                want = ranking.sample(s, u, temperature=T, top_p=p, min_p=m, return_logp=True)
+                got = ranking.sample(s, u, temperature=full(T), top_p=full(p), min_p=full(m), return_logp=True)
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), (T, p, m)
+    for k in (2 ** 32 + 5, 2 ** 40, -(2 ** 35) + 3):  # off
+        assert torch.equal(ranking.sample(s, u, top_k=full(k, torch.int64)), ranking.sample(s, u))
+    assert torch.equal(ranking.sample(s, u, top_k=full(5, torch.int64)), ranking.sample(s, u, top_k=5))

@@ -52,3 +52,16 @@ def test_the_command_refuses(flag, value):
     from regcn_amd import cli
     with pytest.raises(ValueError, match="--sample"):
         cli.main(["-d", "synthetic:icews14s_lgcn_roth", "--test", "--multi-step", "--sample-draws", "4", flag, value])
+
+
+def test_limits_per_row_are_not_narrowed():
+    limit = lambda v, whole: ranking._limit(v, "it", len(v), v.device, whole, 0, 1)[1]  # noqa: E731
+    got = limit(torch.tensor([2 ** 32 + 5, -2 ** 40, 2 ** 31 - 1, -1, 7]), True)
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, 0, 2 ** 31 - 1, 0, 7]
+    assert limit(torch.tensor([5, 100], dtype=torch.int8), True).tolist() == [5, 100]
+    assert limit(torch.tensor([float("nan"), float("inf"), 3.0, -2.0]), True).tolist() == [0, 2 ** 30, 3, 0]
+    fine = torch.tensor([0.9, 1e-50], dtype=torch.float64)
+    assert torch.equal(limit(fine, False), fine) and limit(fine, False).dtype == torch.float64
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        assert limit(fine.to(dt), False).dtype == torch.float32 and torch.equal(limit(fine.to(dt), False), fine.to(dt).float())
+    assert limit(torch.tensor([2 ** 24 + 1]), False).tolist() == [2 ** 24 + 1]
