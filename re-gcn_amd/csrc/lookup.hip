@@ -35,6 +35,7 @@ constexpr int ROW_THR = 256;
 constexpr int64_t STREAM_BYTES = 16 << 20;
 constexpr int MAX_ROWS = 512;      // rows a workgroup of k_row_grads
 constexpr int DEAL = 32;           // workgroups that share out their rows
+constexpr int GRID_Y = 65535;      // most workgroups along a launch's second dimension
 constexpr int SLICE = 16;          // 16-byte pieces of the columns a workgroup of k_partials takes
 
 struct Tokens {
@@ -272,7 +273,7 @@ struct Levels {
 template <typename T, int LO>
 __global__ __launch_bounds__(ROW_THR) void k_partials(const T* __restrict__ g, const int32_t* __restrict__ perm,
                                                       const uint32_t* __restrict__ skey, int64_t n, int64_t V, int d,
-                                                      int64_t dp, int2* __restrict__ runs, Levels lv) {
+                                                      int64_t dp, int per, int slice0, int2* __restrict__ runs, Levels lv) {
   constexpr int VE = Piece<T>::VE;
   constexpr int64_t NODE = LO == 0 ? FAN : (int64_t)FAN * FAN * FAN;  // tokens of a node of level LO + 1
   const int64_t p0 = (int64_t)blockIdx.x * NODE * FAN;
@@ -295,8 +296,7 @@ __global__ __launch_bounds__(ROW_THR) void k_partials(const T* __restrict__ g, c
     full[threadIdx.x] = q + NODE <= n && skey[q] < V && skey[q] == skey[q + NODE - 1];
   }
   __syncthreads();
-  const int per = ((int)(dp / VE) + gridDim.y - 1) / gridDim.y;  // this workgroup's pieces of the columns
-  const int slice = blockIdx.y * per;
+  const int slice = (slice0 + blockIdx.y) * per;  // this workgroup's `per` pieces of the columns
   const int C = min((int)(dp / VE) - slice, per);
   const int64_t node0 = (int64_t)blockIdx.x * FAN;
   const int b = threadIdx.x / SLICE, c0 = (slice + threadIdx.x % SLICE) * VE;
@@ -411,7 +411,7 @@ GradWs grad_ws(int64_t n, int64_t V, int d, void* ws) {
 
 int check_common(const char* what, const void* idx, int64_t n, int64_t V, int d, int dtype) {
   if (d <= 0 || n < 0 || V < 0) return set_error(REGCN_EINVAL, "%s: bad size (n=%lld V=%lld d=%d)", what, (long long)n, (long long)V, d);
-  if (n > 0x7fffffff - 1024 || V >= 0x7fffffff) return set_error(REGCN_ENOTSUP, "%s: n and V below 2^31", what);
+  if (n > 0x7fffffff - 1024 || V >= 0x7fffffff || d > 0x7fffffff - 1024) return set_error(REGCN_ENOTSUP, "%s: n, V and d below 2^31 - 1023", what);
   if (dtype < REGCN_F32 || dtype > REGCN_F16) return set_error(REGCN_EINVAL, "%s: bad element type %d", what, dtype);
   if (n > 0 && !idx) return set_error(REGCN_EINVAL, "%s: null index", what);
   return 0;
@@ -457,11 +457,15 @@ int launch_grad(const void* g, const Tokens& t, int d, float scale, void* out, c
   const int32_t* perm = w.val[side];
   static_assert(FAN == 16, "levels by shifts of 4");
   const int slices = (int)((w.dp / VE + SLICE - 1) / SLICE);
-  if (n > 0)
-    k_partials<T, 0><<<dim3((int)((n + FAN * FAN - 1) / (FAN * FAN)), slices), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp,
-                                                                                  w.runs, w.lv);
-  if (n >> 12)
-    k_partials<T, 2><<<dim3((int)((n + 65535) / 65536), slices), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, w.runs, w.lv);
+  const int per = ((int)(w.dp / VE) + slices - 1) / slices;
+  for (int y0 = 0; n > 0 && y0 < slices; y0 += GRID_Y) {  // (one launch each up to a row of 4 M fp32)
+    const int ys = std::min(slices - y0, GRID_Y);
+    k_partials<T, 0><<<dim3((int)((n + FAN * FAN - 1) / (FAN * FAN)), ys), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, per,
+                                                                                             y0, w.runs, w.lv);
+    if (n >> 12)
+      k_partials<T, 2><<<dim3((int)((n + 65535) / 65536), ys), ROW_THR, 0, st>>>((const T*)g, perm, skey, n, V, d, w.dp, per, y0, w.runs,
+                                                                                  w.lv);
+  }
   const int C = (d + VE - 1) / VE;
   // rows a workgroup: enough for its 256 threads, up to 2048 pieces while that leaves 2048 workgroups
   const int64_t want = std::min<int64_t>(2048, std::max<int64_t>(ROW_THR, V * C / 2048));

@@ -35,6 +35,9 @@ constexpr int ROW_MAX = 32768;  // scores of a row held in LDS
 constexpr int LIST = 256;       // members of a bin that are put in order one against the other
 constexpr int SEG = 8192, SEG_THR = 512;
 constexpr int MAX_COLS = 1 << 24;
+// A launch has fewer than 2^32 threads along a dimension: rows (up to 1024 threads each) and draws (SEG_THR) of one.
+constexpr int LAUNCH_ROWS = 1 << 21, LAUNCH_DRAWS = 1 << 22;
+constexpr int MAX_DRAWS = 1 << 30;
 constexpr uint32_t ALL = 0xffffffffu;
 constexpr int NO_TIE = 0x7fffffff;
 constexpr float LOWEST = -3.402823466e+38f;
@@ -661,7 +664,7 @@ struct Spread {
   RowState* state;
   uint64_t* seg_sum;  // rows x segs
   Member* list;       // rows x cap
-  int segs, cap;
+  int segs, cap, draw0;
   int per;  // segments a workgroup of the range, histogram and member launches
 };
 
@@ -868,7 +871,7 @@ __global__ __launch_bounds__(SEG_THR) void k_spread_draw(Spread p) {
   __shared__ uint64_t found_run;
   __shared__ int found;
   const int r = blockIdx.y;
-  const int64_t at = (int64_t)r * p.a.draws + blockIdx.x;
+  const int64_t at = (int64_t)r * p.a.draws + p.draw0 + blockIdx.x;
   if (p.state[r].kmax == 0) {
     if (threadIdx.x == 0) store_none(p.a, at);
     return;
@@ -959,31 +962,37 @@ int launch_spread(const RowArgs& a, void* ws, hipStream_t st) {
   if (a.top_k_v || (a.top_k > 0 && a.top_k < a.cols) || a.temperature_v || !(a.temperature > 0)) launch_cut<T, false>(p, st);
   if (a.top_p_v || a.top_p < 1.0) launch_cut<T, true>(p, st);
   k_spread_sums<T><<<grid, SEG_THR, 0, st>>>(p);
-  k_spread_draw<T><<<dim3(a.draws, a.rows), SEG_THR, 0, st>>>(p);
+  for (; p.draw0 < a.draws; p.draw0 += LAUNCH_DRAWS)
+    k_spread_draw<T><<<dim3(std::min(a.draws - p.draw0, LAUNCH_DRAWS), a.rows), SEG_THR, 0, st>>>(p);
   return check_launch("sample");
 }
 
 template <typename T>
-int dispatch(const RowArgs& a, void* ws, hipStream_t st) {
+int launch_rows(const RowArgs& a, void* ws, hipStream_t st) {
   if (a.cols <= 2048) return launch<T, 256, 2048>(a, st);
   if (a.cols <= 8192) return launch<T, 512, 8192>(a, st);
   if (a.cols <= 16384) return launch<T, 1024, 16384>(a, st);
   if (a.cols <= 24576) return launch<T, 1024, 24576>(a, st);
   if (a.cols <= ROW_MAX) return launch<T, 1024, ROW_MAX>(a, st);
+  return launch_spread<T>(a, ws, st);
+}
+
+template <typename T>
+int dispatch(const RowArgs& a, void* ws, hipStream_t st) {
   RowArgs part = a;
   const auto from = [&](const void* v, int wide, int64_t r0) { return v ? (const char*)v + r0 * (wide ? 8 : 4) : nullptr; };
-  const int most = rows_at_once(a.cols);
-  for (int r0 = 0; r0 < a.rows; r0 += most) {
-    part.rows = std::min(most, a.rows - r0);
-    part.score = (const T*)a.score + (int64_t)r0 * a.ld;
-    part.u = (const char*)a.u + (int64_t)r0 * a.draws * (a.u_wide ? 8 : 4);
-    part.ids = a.ids + (int64_t)r0 * a.draws;
-    part.logp = a.logp ? a.logp + (int64_t)r0 * a.draws : nullptr;
+  const int most = a.cols <= ROW_MAX ? LAUNCH_ROWS : rows_at_once(a.cols);
+  for (int64_t r0 = 0; r0 < a.rows; r0 += most) {
+    part.rows = (int)std::min<int64_t>(most, a.rows - r0);
+    part.score = (const T*)a.score + r0 * a.ld;
+    part.u = (const char*)a.u + r0 * a.draws * (a.u_wide ? 8 : 4);
+    part.ids = a.ids + r0 * a.draws;
+    part.logp = a.logp ? a.logp + r0 * a.draws : nullptr;
     part.temperature_v = from(a.temperature_v, a.rows_wide & 1, r0);
     part.top_k_v = a.top_k_v ? a.top_k_v + r0 : nullptr;
     part.top_p_v = from(a.top_p_v, a.rows_wide & 2, r0);
     part.min_p_v = from(a.min_p_v, a.rows_wide & 4, r0);
-    if (int rc = launch_spread<T>(part, ws, st)) return rc;
+    if (int rc = launch_rows<T>(part, ws, st)) return rc;
   }
   return 0;
 }
@@ -1000,6 +1009,7 @@ int sample(const regcn_sample_desc& d, hipStream_t st) {
   if (d.rows < 0 || d.cols < 0 || d.draws < 0) return set_error(REGCN_EINVAL, "sample: negative size");
   if (d.dtype < REGCN_F32 || d.dtype > REGCN_F16) return set_error(REGCN_EINVAL, "sample: bad element type %d", d.dtype);
   if (d.cols > MAX_COLS) return set_error(REGCN_ENOTSUP, "sample: rows of up to %d scores", MAX_COLS);
+  if (d.draws > MAX_DRAWS) return set_error(REGCN_ENOTSUP, "sample: up to %d draws a row", MAX_DRAWS);
   if (!d.ids || !d.u || (d.cols > 0 && !d.score)) return set_error(REGCN_EINVAL, "sample: null score, u or ids");
   if (d.rows > 1 && d.ld < d.cols) return set_error(REGCN_EINVAL, "sample: row stride %lld below cols=%d", (long long)d.ld, d.cols);
   if (d.rows == 0 || d.draws == 0) return 0;

@@ -862,18 +862,19 @@ def embedding(table, idx, scale=1.0, padding_idx=None):
         raise TypeError("table must be float32, bfloat16 or float16 (got %s)" % table.dtype)
     if idx.dtype not in (torch.int64, torch.int32):
         raise TypeError("idx must be int64 or int32 (got %s)" % idx.dtype)
+    V = table.shape[0]
+    if V >= 2 ** 31 - 1 or max(idx.numel(), table.shape[1]) > 2 ** 31 - 1025:
+        raise ValueError("embedding takes fewer than 2^31 rows, columns and tokens (got %d, %d, %d)"
+                         % (V, table.shape[1], idx.numel()))
     if not table.is_cuda or idx.device != table.device:
         raise ValueError("table and idx must live on one HIP device (got %s, %s); the HIP path has no CPU fallback"
                          % (table.device, idx.device))
-    V = table.shape[0]
     pad = -1
     if padding_idx is not None:
         pad = int(padding_idx)
         if not -V <= pad < V:
             raise ValueError("padding_idx %d is outside the table's %d rows" % (pad, V))
         pad %= V
-    if V >= 2 ** 31 - 1 or idx.numel() > 2 ** 31 - 1025:
-        raise ValueError("embedding takes fewer than 2^31 rows and tokens (got %d, %d)" % (V, idx.numel()))
     scale = float(scale)
     idx = idx.contiguous()
     if table.shape[1] > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < table.shape[1]:

@@ -88,6 +88,7 @@ def get_total_rank(test_triples, score, all_ans, eval_bz, rel_predict=0):
 
 
 _SAMPLE_MAX_COLS = 1 << 24
+_SAMPLE_MAX_DRAWS = 1 << 30
 
 
 def _row_limits(value, whole):
@@ -146,6 +147,9 @@ def sample(score, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp
     cols = score.shape[-1]
     if cols > _SAMPLE_MAX_COLS:
         raise ValueError("rows of up to %d scores (got %d)" % (_SAMPLE_MAX_COLS, cols))
+    if rows > 2 ** 31 - 1 or rows and u.numel() // rows > _SAMPLE_MAX_DRAWS:
+        raise ValueError("fewer than 2^31 rows and up to %d draws a row (got %d, %d)"
+                         % (_SAMPLE_MAX_DRAWS, rows, u.numel() // rows))
     dev = score.device
     t, t_rows = _limit(temperature, "temperature", rows, dev, False, 0.0, float("inf"), False)
     k, k_rows = _limit(top_k, "top_k", rows, dev, True, 0, 2 ** 31 - 1)

@@ -46,3 +46,17 @@ def test_c_entries_refuse():
 def test_workspace_grows(n, V, d):
     f = _lib.lib().regcn_embedding_grad_workspace_bytes
     assert 0 < f(n, V, d) <= f(n + 1, V, d) <= f(n + 1, V + 100, d + 8)
+
+
+@pytest.mark.parametrize("shape,n", [((1, 1 << 31), 3), ((1 << 31, 1), 3), ((4, 8), 1 << 31), ((1, (1 << 32) + 5), 3)])
+def test_sizes_past_int32_are_refused(shape, n):
+    """Not passed on as what is left of them in 32 bits."""
+    with pytest.raises(ValueError, match="fewer than 2\\^31"):
+        A.embedding(torch.zeros(1, 1).expand(shape), torch.zeros(1, dtype=torch.int64).expand(n))
+
+
+def test_c_entries_refuse_wide_rows():
+    lib = _lib.lib()
+    p = ctypes.addressof(ctypes.create_string_buffer(4096))
+    assert lib.regcn_embedding(p, 0x7fffffff, p, 1, 4, 16, 0x7fffffff, 0, 1.0, p, None) < 0
+    assert lib.regcn_embedding_grad(p, p, 1, 4, 16, 0x7fffffff, -1, 0, 1.0, p, p, 1 << 62, None) < 0

@@ -261,3 +261,17 @@ def test_large_offsets():
     assert float((grad[used].double().cpu() - ref).abs().max()) <= 2.0 ** -8 * float(ref.abs().max())
     grad[used] = 0
     assert not bool(grad.any())
+
+
+@pytest.mark.parametrize("d,dt", [(4_400_001, F32), (8_500_000, BF16)])
+def test_rows_wider_than_a_launch_holds(d, dt):
+    """More column slices than a launch's second dimension holds; whole numbers, so exact sums."""
+    idx = torch.tensor([2] * 70 + [0] * 300 + [1], device=DEV)
+    g = torch.randint(-1, 2, (len(idx), 1), device=DEV).to(dt)
+    table = torch.zeros(3, d, device=DEV, dtype=dt, requires_grad=True)
+    wide = torch.arange(d, device=DEV).remainder(3).sub(1).to(dt)
+    wide[:300] = 0
+    wide[-5:] = 1
+    grad, = torch.autograd.grad(A.embedding(table, idx), table, g * wide)
+    count = torch.zeros(3, device=DEV).index_add_(0, idx, g[:, 0].float())
+    assert torch.equal(grad.float(), count[:, None] * wide.float())

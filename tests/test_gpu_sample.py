@@ -270,3 +270,21 @@ def test_limits_per_row_in_64_bits(N):
     for k in (2 ** 32 + 5, 2 ** 40, -(2 ** 35) + 3):  # off
         assert torch.equal(ranking.sample(s, u, top_k=full(k, torch.int64)), ranking.sample(s, u))
     assert torch.equal(ranking.sample(s, u, top_k=full(5, torch.int64)), ranking.sample(s, u, top_k=5))
+
+
+def test_more_rows_and_draws_than_a_launch_holds():
+    """18 million rows of 3 scores; 9 million draws from a row of 40,000: each takes more than one launch."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    s = torch.rand(18_000_001, 3, device=DEV, generator=gen)
+    u = torch.rand(18_000_001, device=DEV, generator=gen)
+    assert torch.equal(ranking.sample(s, u, top_k=1), s.argmax(1))
+    T = torch.where(torch.arange(18_000_001, device=DEV) % 2 == 0, 0.0, 1e-6)  # both: one of the best, others are 1 below
+    far = (s * 1e4).round()
+    first = ranking.sample(far, u, temperature=T)
+    assert bool((far.gather(1, first[:, None])[:, 0] == far.amax(1)).all())
+    del s, u, far, first
+    row = torch.zeros(40000, device=DEV)
+    n = 9_000_000
+    u = (torch.arange(n, dtype=torch.float64, device=DEV) + 0.5) / n
+    got = ranking.sample(row, u)  # equal weights: the place of u in the row, to the weight's rounding
+    assert torch.equal(got, (u * 40000).long())

@@ -65,3 +65,16 @@ def test_limits_per_row_are_not_narrowed():
     for dt in (torch.float32, torch.float16, torch.bfloat16):
         assert limit(fine.to(dt), False).dtype == torch.float32 and torch.equal(limit(fine.to(dt), False), fine.to(dt).float())
     assert limit(torch.tensor([2 ** 24 + 1]), False).tolist() == [2 ** 24 + 1]
+
+
+def test_sizes_past_int32_are_refused():
+    """Not passed on as what is left of them in 32 bits."""
+    one = torch.zeros(1, 1)
+    for score, u in ((one.expand(1 << 31, 1), torch.zeros(1).expand(1 << 31)), (one, one.expand(1, (1 << 30) + 1)),
+                     (one, one.expand(1, (1 << 32) + 1)), (one[0], one[0].expand((1 << 30) + 1))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ranking.sample(score, u)
+    lib = _lib.lib()
+    p = ctypes.addressof(ctypes.create_string_buffer(4096))
+    d = _lib.SampleDesc(score=p, u=p, ids=p, ld=10, rows=1, cols=10, draws=(1 << 30) + 1, temperature=1.0, top_p=1.0)
+    assert lib.regcn_sample(ctypes.byref(d), None) < 0
