@@ -275,3 +275,34 @@ def test_rows_wider_than_a_launch_holds(d, dt):
     grad, = torch.autograd.grad(A.embedding(table, idx), table, g * wide)
     count = torch.zeros(3, device=DEV).index_add_(0, idx, g[:, 0].float())
     assert torch.equal(grad.float(), count[:, None] * wide.float())
+
+
+def test_forward_mode():
+    """The lookup is linear in the table and its gradient in g: their tangents are the same maps of the tangents."""
+    from torch.autograd import forward_ad
+    V, d = 30, 12
+    table, tangent = torch.randn(V, d, device=DEV), torch.randn(V, d, device=DEV)
+    idx = tokens(V, 50, 1, "flat").to(DEV)
+    for t, v in ((table, tangent), (table.clone().requires_grad_(True), tangent), (table.t().contiguous().t(), tangent.t().contiguous().t())):
+        with forward_ad.dual_level():
+            out = A.embedding(forward_ad.make_dual(t, v), idx, 0.5)
+            primal, got = forward_ad.unpack_dual(out)
+            assert torch.equal(primal.detach(), table[idx] * 0.5)
+            assert got is not None and torch.equal(got.detach(), tangent[idx] * 0.5)
+            assert forward_ad.unpack_dual(A.embedding(table, idx)).tangent is None
+    f = lambda t: A.embedding(t, idx, 0.5, padding_idx=3)  # noqa: E731
+    out, got = torch.func.jvp(f, (table,), (tangent,))
+    assert torch.equal(out, table[idx] * 0.5) and torch.equal(got, tangent[idx] * 0.5)
+    g = torch.randn(50, d, device=DEV)
+    leaf = table.clone().requires_grad_(True)
+    want, = torch.autograd.grad(f(leaf), leaf, g)
+    assert torch.equal(torch.func.vjp(f, table)[1](g)[0], want)
+    assert torch.equal(torch.func.grad(lambda t: (f(t) * g).sum())(table), want)
+    # forward over reverse: the gradient of sum(f(t)^3) / 3 along the tangent
+    with forward_ad.dual_level():
+        leaf = table.clone().requires_grad_(True)
+        dual = forward_ad.make_dual(leaf, tangent)
+        grad, = torch.autograd.grad((f(dual) ** 3).sum() / 3, leaf, create_graph=True)
+        got = forward_ad.unpack_dual(grad).tangent
+    y, dy = (table[idx] * 0.5).double(), (tangent[idx] * 0.5).double()
+    check_grad(got.detach(), 2 * y * dy, idx, 0.5, pad=3)
