@@ -37,6 +37,8 @@ extern "C" {
 #define REGCN_F32 0
 #define REGCN_BF16 1
 #define REGCN_F16 2
+/* Or-ed to a matrix's type (regcn_orthogonalize): its operands stay fp32. */
+#define REGCN_FULL_FP32 0x100
 
 /* Snapshot work lists built by the host (re-gcn_amd/regcn_amd/graph.py):
  * chunks: int32[n_chunks][4] = {row, edge_begin, edge_end, slot}; slot < 0 means
@@ -869,9 +871,13 @@ typedef struct regcn_matrix {
   int32_t dtype;
 } regcn_matrix;
 /* Newton-Schulz iteration of each matrix on its shorter side: X = G / (|G|_F + eps), then `steps` times
- * A = X X^T, X = a X + (b A + c A A) X, as exact as fp32 products, one rounding to the result's type.
+ * A = X X^T, X = a X + (b A + c A A) X, one rounding to the result's type.  The products are as exact as fp32 ones,
+ * on operands of 22 bits (two fp16 halves) that keep nothing below 2^-37 of the matrix's norm: the result's error is
+ * fp32's in the norm of the whole, but rows 1e-4, 1e-5, 1e-6 of the others are off by 4e-6, 4e-5, 4e-4 of themselves.
+ * Matrices of up to 64 rows or columns and those with REGCN_FULL_FP32 keep fp32 operands; more than 8 steps of larger ones
+ * are refused without it (REGCN_ENOTSUP).
  * a, b, c must keep the iteration of a singular value, s <- a s + b s^3 + c s^5 from [0, 1], within
- * |s| <= 2 and |b s^2 + c s^4| <= 16: the operands are held in fp16 halves.  `mats` is host memory and read before the call returns. */
+ * |s| <= 2 and |b s^2 + c s^4| <= 16.  `mats` is host memory and read before the call returns. */
 int64_t regcn_orthogonalize_workspace_bytes(const regcn_matrix* mats, int32_t n_mats);
 int regcn_orthogonalize(const regcn_matrix* mats, int32_t n_mats, int32_t steps, float a, float b, float c, float eps,
                         void* workspace, size_t ws_bytes, void* stream);

@@ -20,6 +20,11 @@
 // fp32 is by 0.3 to 1.4e-6; from 100 x 200 on halves are the closer ones (200 x 200: 1.2e-6, 1.6e-6).  Their
 // products are short, so it costs little: 3 x 30 71 -> 75 us, 64 x 1024 107 -> 136, 64 x 10000 139 -> 148.
 //
+// What the halves do not keep: X's 2^-37 is absolute, so a row of G that is 1e-4, 1e-5 or 1e-6 of the others is off by 4e-6,
+// 4e-5, 4e-4 of itself (fp32: 3e-7), at any number of steps.  Of the whole matrix that is nothing until the small
+// rows have grown by a^steps: the halves' error, modelled in 64 bits over rows of 1 to 1e-8, is 0.3 to 0.7 of fp32's up to 8
+// steps, 4 times it at 10, 40 at 12.  So more than 8 steps take fp32 operands, and a caller may ask for them (REGCN_FULL_FP32).
+//
 // Layout of an operand: rows of 8-element groups, each group 8 hi then 8 lo halves (or 8 fp32): a tile's k-step of
 // 32 is one 128-byte line of a row.  Rows and columns are padded to the tile with zeros, which
 // stay zero through every product, so the inner loop has no bounds.
@@ -33,6 +38,8 @@ namespace regcn {
 namespace {
 
 constexpr int MAXM = 32;      // matrices in a set of launches
+constexpr int FP32_ROWS = 64;  // of matrices that stay in fp32
+constexpr int SPLIT_STEPS = 8;  // most steps of operands in halves
 constexpr int THR = 256;
 constexpr int KSTEP = 32;     // k of a stage: a 128-byte line of each row
 constexpr int NORM_WGS = 1024;  // most partial sums of a norm
@@ -52,6 +59,7 @@ struct Mat {
     int32_t full, splits;  // whole tiles, pieces of k of the others
   } gram, poly;
   int32_t sym;      // tile of the symmetric products
+  int32_t fp32;     // operands held in fp32: tiles of 64
 };
 
 struct Job {
@@ -147,9 +155,6 @@ __global__ __launch_bounds__(THR) void k_norm(Job job) {
   if (threadIdx.x == 0) ((double*)(q.ws + Parts<T>(q).norm))[wg] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-// A matrix held in fp32: its tile is 64 and it is one row of tiles.
-__host__ __device__ inline bool in_fp32(const Mat& q, int tile) { return tile == 64 && q.m <= 64; }
-
 // 8 numbers as a group: 8 hi, 8 lo, or 8 fp32.
 __device__ __forceinline__ void store_group(char* p, const float (&v)[8], bool fp32) {
   if (fp32) {
@@ -227,10 +232,10 @@ __global__ __launch_bounds__(THR) void k_split(Job job) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[r][8 * g + e];
-    store_group(X + (int64_t)r * w.np * 4 + g * 32, v, in_fp32(q, T));
+    store_group(X + (int64_t)r * w.np * 4 + g * 32, v, T == 64 && q.fp32);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[8 * g + e][r];
-    store_group(XT + (int64_t)r * w.mp * 4 + g * 32, v, in_fp32(q, T));
+    store_group(XT + (int64_t)r * w.mp * 4 + g * 32, v, T == 64 && q.fp32);
   }
 }
 
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(THR, 2) void k_gram(Job job) {
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
   const int nt = w.mp / T;
-  symmetric<S>(in_fp32(q, PAD), symmetric_piece(wg, nt, q.gram.full, q.gram.splits, T == 128), q.gram.splits, q.ws + w.x, (int64_t)w.np * 4,
+  symmetric<S>(PAD == 64 && q.fp32, symmetric_piece(wg, nt, q.gram.full, q.gram.splits, T == 128), q.gram.splits, q.ws + w.x, (int64_t)w.np * 4,
                w.np / KSTEP, nullptr, 0.f, 1.f / EX, q.ws + w.A, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
                nt * (nt + 1) / 2 - q.gram.full, lds);
 }
@@ -591,7 +596,7 @@ __global__ __launch_bounds__(THR) void k_gram_sum(Job job) {
   int wg = blockIdx.x;
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
-  symmetric_sum<T>(in_fp32(q, PAD), wg, w.mp / T, q.gram.full, q.gram.splits, (const float*)(q.ws + w.split), nullptr, 0.f, 1.f / EX,
+  symmetric_sum<T>(PAD == 64 && q.fp32, wg, w.mp / T, q.gram.full, q.gram.splits, (const float*)(q.ws + w.split), nullptr, 0.f, 1.f / EX,
                    q.ws + w.A, (int64_t)w.mp * 4, c);
 }
 
@@ -605,7 +610,7 @@ __global__ __launch_bounds__(THR, 2) void k_poly(Job job) {
   const Parts<PAD> w(q);
   const int nt = w.mp / T;
   const char* A = q.ws + w.A;
-  symmetric<S>(in_fp32(q, PAD), symmetric_piece(wg, nt, q.poly.full, q.poly.splits, T == 128), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
+  symmetric<S>(PAD == 64 && q.fp32, symmetric_piece(wg, nt, q.poly.full, q.poly.splits, T == 128), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
                job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
                nt * (nt + 1) / 2 - q.poly.full, lds);
 }
@@ -615,7 +620,7 @@ __global__ __launch_bounds__(THR) void k_poly_sum(Job job) {
   int wg = blockIdx.x;
   const Mat& q = job.mat[find_mat(job, wg)];
   const Parts<PAD> w(q);
-  symmetric_sum<T>(in_fp32(q, PAD), wg, w.mp / T, q.poly.full, q.poly.splits, (const float*)(q.ws + w.split), q.ws + w.A,
+  symmetric_sum<T>(PAD == 64 && q.fp32, wg, w.mp / T, q.poly.full, q.poly.splits, (const float*)(q.ws + w.split), q.ws + w.A,
                    job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, c);
 }
 
@@ -632,7 +637,7 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
   char* const ws = q.ws;
   void* const result = q.out;
   const int m = q.m, n = q.n, dtype = q.dtype;
-  const bool trans = q.trans, fp32 = in_fp32(q, T);
+  const bool trans = q.trans, fp32 = T == 64 && q.fp32;
   const int mt = w.mp / T;
   wg = by_xcd(wg, mt * (w.np / T));
   const int i0 = wg % mt * T, j0 = wg / mt * T;
@@ -655,6 +660,7 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 2) void k_update(Job job) {
 // 128 tiles of 256, 1,125 us in tiles of 128 and 1,266 of 256; 2900 x 2900, 144 tiles, 2,012 and 1,888; 1536 x 1536,
 // 144 tiles of 128, 589 us and 447 in 64; 2048 x 4096, 512 tiles, 1,125 and 1,229.
 int tile_of(const Mat& q) {
+  if (q.fp32) return 64;
   const auto tiles = [&](int t) { return q.m > t / 2 ? (int64_t)((q.m + t - 1) / t) * ((q.n + t - 1) / t) : 0; };
   return tiles(256) >= 136 ? 256 : tiles(128) >= 192 ? 128 : 64;
 }
@@ -721,18 +727,20 @@ int64_t mat_bytes(const Mat& q) {
 int to_mat(const regcn_matrix& d, Mat& q) {
   if (d.rows <= 0 || d.cols <= 0) return set_error(REGCN_EINVAL, "orthogonalize: bad size %lld x %lld", (long long)d.rows, (long long)d.cols);
   if (d.rows > (1 << 20) || d.cols > (1 << 20)) return set_error(REGCN_ENOTSUP, "orthogonalize: sides up to 2^20");
-  if (d.dtype < REGCN_F32 || d.dtype > REGCN_F16) return set_error(REGCN_EINVAL, "orthogonalize: bad element type %d", d.dtype);
+  const int dtype = d.dtype & ~REGCN_FULL_FP32;
+  if (dtype < REGCN_F32 || dtype > REGCN_F16) return set_error(REGCN_EINVAL, "orthogonalize: bad element type %d", d.dtype);
   q = Mat{};
   q.g = d.x;
   q.out = d.out;
   q.trans = d.rows > d.cols;
   q.m = (int)std::min(d.rows, d.cols);
   q.n = (int)std::max(d.rows, d.cols);
-  q.dtype = d.dtype;
+  q.dtype = dtype;
+  q.fp32 = q.m <= FP32_ROWS || (d.dtype & REGCN_FULL_FP32) != 0;
   if ((int64_t)q.m * q.n > (1ll << 40)) return set_error(REGCN_ENOTSUP, "orthogonalize: up to 2^40 elements");
   const int t = tile_of(q), st = q.sym = sym_tile_of(q, t), nt = pad_to(q.m, t) / st, tri = nt * (nt + 1) / 2;
-  q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP, in_fp32(q, t));
-  q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP, in_fp32(q, t));
+  q.gram = cut_of(tri, pad_to(q.n, t) / KSTEP, q.fp32);
+  q.poly = cut_of(tri, pad_to(q.m, t) / KSTEP, q.fp32);
   return 0;
 }
 
@@ -778,6 +786,8 @@ int orthogonalize(const regcn_matrix* mats, int count, int steps, float a, float
   for (int k = 0; k < count; ++k) {
     Mat q;
     if (int rc = to_mat(mats[k], q)) return rc;
+    if (steps > SPLIT_STEPS && !q.fp32)
+      return set_error(REGCN_ENOTSUP, "orthogonalize: more than %d steps take REGCN_FULL_FP32 (matrix %d)", SPLIT_STEPS, k);
     if (!mats[k].x || !mats[k].out) return set_error(REGCN_EINVAL, "orthogonalize: null matrix %d", k);
   }
   const int64_t need = orthogonalize_ws_bytes(mats, count);

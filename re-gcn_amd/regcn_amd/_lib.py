@@ -116,6 +116,7 @@ _SIGS = {
 }
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # REGCN_F32, REGCN_BF16, REGCN_F16
+FULL_FP32 = 0x100  # REGCN_FULL_FP32
 
 SCORE_DIST, SCORE_RAW_SCALE = 1, 2
 _RESTYPE = {"regcn_last_error_string": ctypes.c_char_p, "regcn_hyp_ce_workspace_bytes": _c_sz,

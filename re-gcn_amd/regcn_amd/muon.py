@@ -5,7 +5,7 @@
     X = G / (|G|_F + eps);   A = X X^T,  X = a X + (b A + c A A) X,   `steps` times,
 
 on a matrix's shorter side, for any number of matrices of any shapes in one set of launches
-(regcn_orthogonalize): the products run on the fp16 matrix cores as exactly as fp32 products.  With the
+(regcn_orthogonalize): the products of operands split into fp16 halves run on the matrix cores.  With the
 default coefficients the singular values end near 1 (0.7 to 1.2), the singular vectors stay.
 """
 import functools
@@ -16,6 +16,7 @@ from . import _lib
 
 COEFFS = (3.4445, -4.7750, 2.0315)
 _LIMIT, _LIMIT_B = 2.0, 16.0
+SPLIT_STEPS = 8  # most steps of operands in halves
 
 
 @functools.lru_cache(maxsize=64)
@@ -47,11 +48,16 @@ def _plan(g):
     return (t, True) if t.is_contiguous() else (g.contiguous(), False)
 
 
-def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7):
+def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, full_fp32=False):
     """Newton-Schulz orthogonalisation of a matrix (m x n), of a stack of them (... x m x n), or of a list
     or tuple of matrices of any shapes and types on one device; the same structure is returned, each result
     in its matrix's type.  An all-zero matrix stays zero (with an eps of 0 it becomes NaN), a matrix without elements is returned as it is;
-    infinities and NaN make their matrix's result NaN.  No gradient flows through the iteration."""
+    infinities and NaN make their matrix's result NaN.  No gradient flows through the iteration.
+
+    Matrices of more than 64 rows and columns are iterated on operands of 22 bits (two fp16 halves) that keep nothing
+    below 2^-37 of the matrix's norm: the error is that of fp32 in the norm of the whole, but rows 1e-4, 1e-5, 1e-6 of the
+    others are off by 4e-6, 4e-5, 4e-4 of themselves.  `full_fp32` keeps fp32 operands, on the fp32 matrix
+    instructions; more than 8 steps always do, since small rows have grown to the others' size by then."""
     steps = int(steps)
     if not 1 <= steps <= 1000:
         raise ValueError("1 to 1000 steps (got %d)" % steps)
@@ -62,21 +68,21 @@ def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7):
         raise ValueError("eps must be a number >= 0 (got %r)" % eps)
     if isinstance(g, torch.Tensor):
         if g.dim() == 2:
-            return _run([g], steps, a, b, c, eps)[0]
+            return _run([g], steps, a, b, c, eps, full_fp32)[0]
         if g.dim() < 2:
             raise ValueError("a matrix has two dimensions (got %s)" % (tuple(g.shape),))
         m, n = g.shape[-2:]
         if g.numel() == 0:
             return g.detach().clone()
-        out = _run(list(g.detach().reshape(-1, m, n).unbind(0)), steps, a, b, c, eps)
+        out = _run(list(g.detach().reshape(-1, m, n).unbind(0)), steps, a, b, c, eps, full_fp32)
         return torch.stack(out).reshape(g.shape)
     if not isinstance(g, (list, tuple)) or not all(isinstance(x, torch.Tensor) for x in g):
         raise TypeError("orthogonalize takes a tensor or a list of matrices (got %s)" % type(g).__name__)
-    out = _run(g, steps, a, b, c, eps)
+    out = _run(g, steps, a, b, c, eps, full_fp32)
     return out if isinstance(g, list) else tuple(out)
 
 
-def _run(mats, steps, a, b, c, eps):
+def _run(mats, steps, a, b, c, eps, full_fp32):
     plans = [_plan(g) for g in mats]
     if not plans:
         return []
@@ -87,10 +93,11 @@ def _run(mats, steps, a, b, c, eps):
     live = [k for k, (p, _) in enumerate(plans) if p.numel()]
     if live:
         desc = (_lib.Matrix * len(live))()
+        flags = _lib.FULL_FP32 if full_fp32 or steps > SPLIT_STEPS else 0
         for d, k in zip(desc, live):
             p = plans[k][0]
             d.x, d.out, d.rows, d.cols, d.dtype = p.data_ptr(), outs[k].data_ptr(), p.shape[0], p.shape[1], \
-                _lib.DTYPES[p.dtype]
+                _lib.DTYPES[p.dtype] | flags
         size = _lib.lib().regcn_orthogonalize_workspace_bytes(desc, len(live))
         ws = torch.empty(size, device=device, dtype=torch.uint8)
         _lib.launch("regcn_orthogonalize", device, desc, len(live), steps, a, b, c, eps, ws.data_ptr(), size)
@@ -110,7 +117,7 @@ class Muon(torch.optim.Optimizer):
     training step with it can be captured in a HIP graph (training.GraphedSteps)."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS,
-                 eps=1e-7):
+                 eps=1e-7, full_fp32=False):
         if not lr >= 0.0:
             raise ValueError("lr must be >= 0 (got %r)" % (lr,))
         if not 0.0 <= momentum < 1.0:
@@ -121,7 +128,7 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("1 to 1000 steps (got %r)" % (steps,))
         _check_coeffs(*(float(v) for v in coeffs), int(steps))
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
-                                      steps=steps, coeffs=tuple(coeffs), eps=eps))
+                                      steps=steps, coeffs=tuple(coeffs), eps=eps, full_fp32=bool(full_fp32)))
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -171,7 +178,7 @@ class Muon(torch.optim.Optimizer):
         if group["nesterov"]:
             d = torch._foreach_mul(bufs, mu)
             torch._foreach_add_(d, grads)
-        o = orthogonalize(d, group["steps"], group["coeffs"], group["eps"])
+        o = orthogonalize(d, group["steps"], group["coeffs"], group["eps"], group.get("full_fp32", False))
         torch._foreach_mul_(o, [max(1.0, p.shape[0] / p.shape[1]) ** 0.5 if p.numel() else 1.0 for p in ps])
         w = [p if p.dtype == torch.float32 else p.float() for p in ps]
         if group["weight_decay"]:

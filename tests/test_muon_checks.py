@@ -71,3 +71,22 @@ def test_muon_refuses_settings(kw):
 def test_muon_refuses_parameters(p):
     with pytest.raises(ValueError):
         muon.Muon([p.requires_grad_(True)])
+
+
+def test_more_steps_take_fp32_operands():
+    """A caller of the C entry asks for them by the matrix's type; the workspace follows."""
+    lib = _lib.lib()
+    p = ctypes.addressof(ctypes.create_string_buffer(4096))
+
+    def mats(rows, dtype):
+        m = (_lib.Matrix * 1)()
+        m[0].x, m[0].out, m[0].rows, m[0].cols, m[0].dtype = p, p, rows, 300, dtype
+        return m
+    size = lambda m: lib.regcn_orthogonalize_workspace_bytes(m, 1)  # noqa: E731
+    call = lambda m, steps: lib.regcn_orthogonalize(m, 1, steps, 1.5, -0.5, 0.0, 0.0, p, 0, None)  # noqa: E731
+    assert call(mats(200, 0), 9) == -2  # REGCN_ENOTSUP
+    assert b"REGCN_FULL_FP32" in lib.regcn_last_error_string()
+    for m, steps in ((mats(200, 0), 8), (mats(200, _lib.FULL_FP32), 9), (mats(64, 0), 9)):
+        assert call(m, steps) == -1 and b"workspace" in lib.regcn_last_error_string()
+    assert size(mats(200, 1 | _lib.FULL_FP32)) > 0 and size(mats(200, 3 | _lib.FULL_FP32)) == 0
+    assert size(mats(64, 0)) == size(mats(64, _lib.FULL_FP32))
