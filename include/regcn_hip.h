@@ -905,8 +905,11 @@ typedef struct regcn_sample_desc {
 /* Per row: weights exp((s - max) / temperature); kept are, in the order "larger score first, ties by lower
  * column", the first top_k, of those the shortest prefix whose weights reach top_p of their sum, and of those
  * the weights >= min_p (the first is always kept); a draw is the lowest column whose running sum (by column)
- * of kept weights exceeds u times their sum.  NaN and -inf scores are never taken; +inf shares all weight. */
-int64_t regcn_sample_workspace_bytes(int32_t rows, int32_t cols, int32_t dtype);
+ * of kept weights exceeds u times their sum.  NaN and -inf scores are never taken; +inf shares all weight.
+ * Weights are rounded to multiples of 2^-S, S = min(51, 63 - ceil(log2 cols)), the largest being 1; their sums are exact.
+ * The rounding moves at most cols 2^-(S+1) of probability (2^-33 at 32768 columns, 2^-24 at 2^20, 2^-16 at 2^24), and a
+ * weight below 2^-(S+1) is never drawn. */
+int64_t regcn_sample_workspace_bytes(int32_t rows, int32_t cols, int32_t dtype); /* the same for every dtype */
 int regcn_sample(const regcn_sample_desc* desc, void* stream);
 
 #ifdef __cplusplus

@@ -8,14 +8,16 @@
 // T <= 0 takes the first of the order.  A row without a score to take gives -1.
 //
 // Weights are whole numbers: round(w 2^S) with 2^S N <= 2^63 (S <= 51), from a 64-bit exp.  Their sums are
-// exact in any order, so histograms by atomics, partial sums and prefix sums agree bit for bit.
+// exact in any order, so histograms by atomics, partial sums and prefix sums agree bit for bit.  What the rounding
+// loses is at most N 2^-(S+1) of the largest weight: 2^-37 at 2,048 scores, 2^-33 at 32,768, 2^-24 at 2^20, 2^-16 at 2^24, where
+// a weight below 2^-40 (28 T under the largest) is 0.
 //
 // No sort.  Each of k and p asks for the place in the order where a running sum (of ones, of weights) reaches
 // a target: a histogram over 2048 bins of the scores finds the bin, whose few members then add up the members
 // before them.  A bin that holds too many (ties, scores far from each other) is cut into bins again, twice in a
 // row held in LDS; then a radix descent over the scores' bits as ordered keys goes on from it, and one over the
 // indices of equal scores.  So a kept set is {score > c} and {score = c, index <= i}.  (3080 x 23033, k = 50 or p = 0.9:
-// 0.2 and 0.37 ms; two different scores 0.7 and 0.8; scores a million T apart 0.6 and 0.25.  16 x 1,000,000: 0.08 and
+// 0.20 and 0.32 ms; two different scores 0.7 and 0.8; scores a million T apart 0.6 and 0.25.  16 x 1,000,000: 0.08 and
 // 0.16 ms, and 1.3 to 1.9 where the descent reads the row, by one workgroup.)
 //
 // k_sample: a workgroup takes a row of up to 32768 scores, which stay in its LDS (one read of them; in
@@ -969,10 +971,11 @@ int launch_spread(const RowArgs& a, void* ws, hipStream_t st) {
 
 template <typename T>
 int launch_rows(const RowArgs& a, void* ws, hipStream_t st) {
+  // As few threads as leave a CU several rows: without the first tier 3080 x 1,000 takes 48 us for 36, without the second
+  // 3080 x 7,128 165 for 90; the third, a row a CU like the last, gains 1.5 % (3080 x 12,000, 109.4 us and 107.6).
   if (a.cols <= 2048) return launch<T, 256, 2048>(a, st);
   if (a.cols <= 8192) return launch<T, 512, 8192>(a, st);
   if (a.cols <= 16384) return launch<T, 1024, 16384>(a, st);
-  if (a.cols <= 24576) return launch<T, 1024, 24576>(a, st);
   if (a.cols <= ROW_MAX) return launch<T, 1024, ROW_MAX>(a, st);
   return launch_spread<T>(a, ws, st);
 }
@@ -1037,8 +1040,10 @@ int sample(const regcn_sample_desc& d, hipStream_t st) {
   a.logp = d.logp;
   a.c.log2e = 1.4426950408889634074;
   a.c.round = 0x1.8p52;
-  a.c.ln2_hi = -6.93147180369123816490e-01;
-  a.c.ln2_lo = -1.90821492927058770002e-10;
+  // ln 2 = 0.693147180559945309417232121458...: its first 32 bits, whose products with a whole number below 2^21 are
+  // exact, and what is left of it
+  a.c.ln2_hi = -2977044471.0 / 4294967296.0;
+  a.c.ln2_lo = -1.908214929270587816e-10;
   double f = 1.0;
   for (int j = 2; j <= 12; ++j) a.c.p[12 - j] = 1.0 / (f *= j);
   int bits = 0;

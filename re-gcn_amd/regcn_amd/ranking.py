@@ -125,10 +125,13 @@ def sample(score, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logp
     weights w = exp((score - max) / temperature): in the order "larger score first, ties by lower id" are
     kept the first `top_k` (0: all), of those the shortest prefix holding `top_p` of their weight, and of
     those w >= `min_p` (the first is always kept); a draw is the lowest id whose running sum, by id, of kept
-    weights exceeds u times their sum.  Sums are exact, so equal inputs give equal ids on every call.
+    weights exceeds u times their sum.  Weights are rounded to multiples of 2^-S, S = min(51, 63 - ceil(log2 N)), and
+    their sums are exact, so equal inputs give equal ids on every call.  The rounding moves at most N 2^-(S+1) of
+    probability: 2^-33 at 32,768 scores, 2^-24 at a million, 2^-16 at the most, 2^24, where scores 28 T below the largest
+    are never drawn.
 
     NaN and -inf scores are never drawn and a row of them gives -1; temperature 0 takes the best id.
-    temperature, top_k, top_p and min_p may each be a tensor of one value per row (not checked: a
+    temperature, top_k, top_p and min_p may each be a tensor of one value per row, fp64 ones in full (not checked: a
     temperature that is not above 0 takes the best id, top_k <= 0, top_p >= 1 and min_p <= 0 are off).
     Returns int64 ids in u's shape, with return_logp also the log of each draw's probability among the
     kept (fp32, -inf where the id is -1)."""

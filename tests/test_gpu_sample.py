@@ -288,3 +288,36 @@ def test_more_rows_and_draws_than_a_launch_holds():
     u = (torch.arange(n, dtype=torch.float64, device=DEV) + 0.5) / n
     got = ranking.sample(row, u)  # equal weights: the place of u in the row, to the weight's rounding
     assert torch.equal(got, (u * 40000).long())
+
+
+@pytest.mark.parametrize("N,dt", [(1 << 20, F32), ((1 << 20) + 1, F16), (3_000_001, F32), (1 << 24, F32)])
+def test_the_widest_rows(N, dt):
+    """Every draw is that of the stated weights, whole multiples of 2^-S: an id's running sum on the host, in whole numbers.
+    The exponentials here are numpy's and may round to another multiple than the kernel's (both within 2^-52, so
+    fewer than N 2^(S-52) of the weights, each by 1): a draw may lie that far over a border.  Against the weights
+    before their rounding it lies within the stated N 2^-(S+1), and again that."""
+    S = min(51, 63 - math.ceil(math.log2(N)))
+    g = torch.Generator().manual_seed(N)
+    s = (torch.rand(N, generator=g) * -33.0).to(dt)
+    s[N // 3], s[5::1000] = 0.0, -30.0
+    u = torch.rand(200, generator=g, dtype=torch.float64)
+    got, logp = ranking.sample(s.to(DEV), u.to(DEV), return_logp=True)
+    w = np.exp(s.double().numpy())
+    whole = np.rint(w * 2.0 ** S).astype(np.uint64)
+    run = np.cumsum(whole)
+    total = int(run[-1])
+    assert total <= 1 << 63
+    slack = max(2, math.ceil(N * 2.0 ** (S - 52)) + 2)
+    exact = np.cumsum(w.astype(np.longdouble))
+    for i, x, lp in zip(got.tolist(), u.tolist(), logp.tolist()):
+        t = x * float(total)
+        assert int(run[i]) - int(whole[i]) - slack <= t + t * 2.0 ** -52 and t - t * 2.0 ** -52 < int(run[i]) + slack
+        assert int(whole[i]) > 0
+        lost = 2.0 * N * 2.0 ** -(S + 1)
+        assert float(exact[i]) - w[i] - lost <= x * float(exact[-1]) <= float(exact[i]) + lost
+        assert abs(lp - (float(s[i]) - math.log(float(exact[-1])))) <= 2.0 ** -24 * abs(lp) * 1.01 + lost / float(exact[-1]) + 2.0 ** -40
+    for lim in (dict(k=1000), dict(p=0.7), dict(k=100000, p=0.5, m=1e-6)):
+        assert torch.equal(ranking.sample(s.to(DEV), u.to(DEV), top_k=lim.get("k", 0), top_p=lim.get("p", 1.0), min_p=lim.get("m", 0.0)),
+                           ranking.sample(s.to(DEV)[None], u.to(DEV)[None], top_k=lim.get("k", 0), top_p=lim.get("p", 1.0),
+                                          min_p=lim.get("m", 0.0))[0])
+        check(s.to(DEV)[None], u.to(DEV)[None], **lim)
