@@ -13,9 +13,9 @@
 // sorted positions, then sums the runs in a fixed order: no atomics, the same bits on every call.
 //   * up to RANK_MAX tokens one launch ranks each token by counting the keys before it;
 //   * more take least-significant-digit radix passes of 10 bits (two launches a pass).
-// A run of any length is summed over a tree of fan 16 on the sorted positions (k_partials: nodes whose
-// tokens all belong to one row); the row's thread adds the at most 15 tokens or nodes at each end of
-// each level, so no chain of dependent loads grows with the run.  Sums are fp32; a 16-bit type is
+// A run of any length is summed over a tree of fan 16 and five levels on the sorted positions (k_partials: nodes whose
+// tokens all belong to one row); the row's thread adds the at most 15 tokens or nodes at each end of each level (30 at the
+// level where a run ends) and, at the last, one node for every 65,536 tokens of the run.  Sums are fp32; a 16-bit type is
 // rounded once, at the store.
 #include "elem.h"
 #include "regcn_internal.h"
