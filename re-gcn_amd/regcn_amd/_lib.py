@@ -270,6 +270,25 @@ def lib():
     return _lib
 
 
+_node = None
+
+
+def node():
+    """The C++ autograd nodes (csrc/node.cpp), bound to this library's entries."""
+    global _node
+    if _node is None:
+        h = lib()
+        try:
+            from . import _node as m
+        except ImportError as e:
+            raise HipLibraryError("the autograd nodes are not built (%s); build them with `python -c \"import __graft_entry__ as "
+                                  "g; g.build()\"`" % e) from e
+        m.bind(*(ctypes.cast(getattr(h, f), ctypes.c_void_p).value for f in (
+            "regcn_embedding", "regcn_embedding_grad_workspace_bytes", "regcn_embedding_grad", "regcn_last_error_string")))
+        _node = m
+    return _node
+
+
 def exported_symbols():
     return list(_SIGS)
 

@@ -811,24 +811,9 @@ def _embedding_sums(g, idx, V, scale, pad):
     return grad
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, idx, scale, pad):
-        ctx.save_for_backward(idx)
-        ctx.V, ctx.scale, ctx.pad = table.shape[0], scale, pad
-        return _embedding_rows(table, idx, scale)
-
-    @staticmethod
-    def backward(ctx, g):
-        (idx,) = ctx.saved_tensors
-        if torch.is_grad_enabled():  # create_graph: the gradient is differentiable in g
-            return _EmbeddingSums.apply(g, idx, ctx.V, ctx.scale, ctx.pad), None, None, None
-        return _embedding_sums(g, idx, ctx.V, ctx.scale, ctx.pad), None, None, None
-
-
 class _EmbeddingTransformed(torch.autograd.Function):
-    """The lookup under forward-mode differentiation and torch.func's transforms (the separate context costs 8 us a
-    call, which the class above spares)."""
+    """The lookup under forward-mode differentiation and torch.func's transforms, and where launches are traced;
+    otherwise its node is csrc/node.cpp's."""
 
     @staticmethod
     def forward(table, idx, scale, pad):
@@ -912,8 +897,9 @@ def embedding(table, idx, scale=1.0, padding_idx=None):
     idx = idx.contiguous()
     if table.shape[1] > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < table.shape[1]:
         table = table.contiguous()
-    if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
+    transformed = forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+    if not transformed and _lib.EVENT_TRACE is None:
+        return _lib.node().lookup(table, idx, scale, pad)
+    if transformed or needs_grad(table):
         return _EmbeddingTransformed.apply(table, idx, scale, pad)
-    if needs_grad(table):
-        return _Embedding.apply(table, idx, scale, pad)
     return _embedding_rows(table.detach(), idx, scale)

@@ -306,3 +306,43 @@ def test_forward_mode():
         got = forward_ad.unpack_dual(grad).tangent
     y, dy = (table[idx] * 0.5).double(), (tangent[idx] * 0.5).double()
     check_grad(got.detach(), 2 * y * dy, idx, 0.5, pad=3)
+
+
+def test_traced_launches():
+    """Under a launch trace the entries are called from Python and show up; the results are the same bits."""
+    from regcn_amd import _lib
+    table, idx = torch.randn(40, 12, device=DEV), tokens(40, 70, 1, "flat").to(DEV)
+    want = both(table, idx, 2.0)
+    plain = A.embedding(table, idx, 2.0)
+    _lib.EVENT_TRACE = []
+    try:
+        got = both(table, idx, 2.0)
+        assert torch.equal(A.embedding(table, idx, 2.0), plain)
+        names = [n for n, _ in _lib.EVENT_TRACE]
+    finally:
+        _lib.EVENT_TRACE = None
+    assert names == ["regcn_embedding", "regcn_embedding_grad", "regcn_embedding"]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_leaves_views_and_modes():
+    """The node's place in a graph: a result without one under no_grad, gradients into views and through two uses."""
+    table, idx = torch.randn(40, 12, device=DEV, requires_grad=True), tokens(40, 70, 1, "flat").to(DEV)
+    with torch.no_grad():
+        assert A.embedding(table, idx).grad_fn is None
+    with torch.inference_mode():
+        assert torch.equal(A.embedding(table, idx), table[idx])
+    assert not A.embedding(table.detach(), idx).requires_grad
+    part = (table * 1.0)[3:30, 2:9]  # rows off 16 bytes, wider apart than long
+    inside = idx.clamp(max=26)
+    out = A.embedding(part, inside) + A.embedding(part, inside.flip(0), 2.0)
+    g = torch.randint(-3, 4, out.shape, device=DEV).float()
+    got, = torch.autograd.grad(out, table, g)
+    ref = table.detach().clone().requires_grad_(True)
+    want, = torch.autograd.grad(ref[3:30, 2:9][inside] + 2.0 * ref[3:30, 2:9][inside.flip(0)], ref, g)
+    assert torch.equal(got, want)  # whole numbers: exact in any order
+    seen = []
+    hooked = A.embedding(table, idx)
+    hooked.register_hook(lambda g: seen.append(g.shape))
+    hooked.sum().backward()
+    assert seen == [(70, 12)] and torch.equal(table.grad[:, 0], torch.bincount(idx, minlength=40).float())
