@@ -1,13 +1,17 @@
-// The embedding lookup's autograd nodes.  A node written in Python runs its backward on the engine's thread, which waits
-// for the interpreter's lock that the calling thread holds.  3,080 tokens of 512 x 200 with their gradient, pass after
-// pass: 84 us with a node in Python, 50 with this one (19 of them the kernels); torch's indexing with its backward takes 76 to
-// 79, a product by 2 with its backward, which is the engine's own cost, 41.
+// Autograd nodes of the embedding lookup and of the relation GRU.  A node written in Python runs its backward on the
+// engine's thread, which waits for the interpreter's lock that the calling thread holds.  3,080 tokens of 512 x 200 with
+// their gradient, pass after pass: 84 us with a node in Python, 50 with this one (19 of them the kernels); torch's indexing
+// with its backward takes 76 to 79, a product by 2 with its backward, which is the engine's own cost, 41.  The GRU's three
+// calls of a training sample: 0.22 ms in Python, 0.1 here.
 //
 // Host code only: the kernels are libregcn_hip.so's, whose entries `bind` is given by the library that Python loaded.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include "../../include/regcn_hip.h"
+
+#include <algorithm>
 #include <cstdint>
 
 namespace {
@@ -18,14 +22,16 @@ using torch::autograd::Function;
 using torch::autograd::variable_list;
 
 struct Entries {
-  int (*lookup)(const void*, int64_t, const void*, int32_t, int64_t, int64_t, int32_t, int32_t, float, void*, void*);
-  int64_t (*grad_bytes)(int64_t, int64_t, int32_t);
-  int (*grad)(const void*, const void*, int32_t, int64_t, int64_t, int32_t, int64_t, int32_t, float, void*, void*, size_t, void*);
-  const char* (*error)();
+  decltype(&regcn_embedding) lookup;
+  decltype(&regcn_embedding_grad_workspace_bytes) grad_bytes;
+  decltype(&regcn_embedding_grad) grad;
+  decltype(&regcn_kreduce_workspace_floats) kreduce_floats;
+  decltype(&regcn_kreduce_gemm_f32) kreduce;
+  decltype(&regcn_last_error_string) error;
 } entry;
 
-int type_of(const Tensor& t) {  // REGCN_F32, REGCN_BF16, REGCN_F16
-  return t.scalar_type() == torch::kFloat ? 0 : t.scalar_type() == torch::kBFloat16 ? 1 : 2;
+int type_of(const Tensor& t) {
+  return t.scalar_type() == torch::kFloat ? REGCN_F32 : t.scalar_type() == torch::kBFloat16 ? REGCN_BF16 : REGCN_F16;
 }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -98,10 +104,38 @@ variable_list Lookup::backward(AutogradContext* ctx, variable_list g) {
           Tensor()};
 }
 
-void bind(uintptr_t lookup, uintptr_t grad_bytes, uintptr_t grad, uintptr_t error) {
+// A GRU cell's gates and new state from its two products, by torch's fused kernels.  Theirs for the backward would sum the
+// biases' gradients on several workgroups, which does not replay in a HIP graph: both are one product with a row of ones here,
+// as autograd.colsum.
+struct GruGates : Function<GruGates> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& gi, const Tensor& gh, const Tensor& h, const Tensor& b_ih, const Tensor& b_hh) {
+    auto [out, ws] = at::_thnn_fused_gru_cell(gi, gh, h, b_ih, b_hh);
+    ctx->save_for_backward({ws});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gy) {
+    const c10::DeviceGuard guard(gy[0].device());
+    auto [di, dh, dx, none_i, none_h] = at::_thnn_fused_gru_cell_backward(gy[0].contiguous(), ctx->get_saved_variables()[0], false);
+    Tensor db;
+    if (ctx->needs_input_grad(3) || ctx->needs_input_grad(4)) {
+      const Tensor both = at::cat({di, dh}, 1), ones = at::ones({both.size(0), 1}, both.options());
+      const int64_t K = both.size(0), N = both.size(1);
+      db = at::empty({2, N / 2}, both.options());
+      const Tensor ws = at::empty({std::max<int64_t>(1, (int64_t)entry.kreduce_floats(K, 1, (int32_t)N))}, both.options());
+      const int rc = entry.kreduce(ones.data_ptr<float>(), 1, both.data_ptr<float>(), 1, K, 1, (int32_t)N, nullptr, 0, db.data_ptr<float>(),
+                                   ws.data_ptr<float>(), stream_of(both));
+      TORCH_CHECK(rc == 0, "regcn_kreduce_gemm_f32 failed (rc=", rc, "): ", entry.error());
+    }
+    return {di, dh, dx, db.defined() ? db[0] : Tensor(), db.defined() ? db[1] : Tensor()};
+  }
+};
+
+void bind(uintptr_t lookup, uintptr_t grad_bytes, uintptr_t grad, uintptr_t kreduce_floats, uintptr_t kreduce, uintptr_t error) {
   entry.lookup = reinterpret_cast<decltype(entry.lookup)>(lookup);
   entry.grad_bytes = reinterpret_cast<decltype(entry.grad_bytes)>(grad_bytes);
   entry.grad = reinterpret_cast<decltype(entry.grad)>(grad);
+  entry.kreduce_floats = reinterpret_cast<decltype(entry.kreduce_floats)>(kreduce_floats);
+  entry.kreduce = reinterpret_cast<decltype(entry.kreduce)>(kreduce);
   entry.error = reinterpret_cast<decltype(entry.error)>(error);
 }
 
@@ -109,7 +143,12 @@ void bind(uintptr_t lookup, uintptr_t grad_bytes, uintptr_t grad, uintptr_t erro
 
 PYBIND11_MODULE(_node, m) {
   m.def("bind", &bind, "Addresses of regcn_embedding, regcn_embedding_grad_workspace_bytes, regcn_embedding_grad, "
-                       "regcn_last_error_string");
+                       "regcn_kreduce_workspace_floats, regcn_kreduce_gemm_f32, regcn_last_error_string");
+  m.def("gru_gates",
+        [](const Tensor& gi, const Tensor& gh, const Tensor& h, const Tensor& b_ih, const Tensor& b_hh) {
+          return GruGates::apply(gi, gh, h, b_ih, b_hh);
+        },
+        "A GRU cell's new state from its two products (fp32, on a HIP device)");
   m.def("lookup", [](const Tensor& table, const Tensor& idx, double scale, int64_t pad) { return Lookup::apply(table, idx, scale, pad); },
         "scale * table[idx] with its gradient; arguments as autograd.embedding has checked them");
 }

@@ -284,7 +284,8 @@ def node():
             raise HipLibraryError("the autograd nodes are not built (%s); build them with `python -c \"import __graft_entry__ as "
                                   "g; g.build()\"`" % e) from e
         m.bind(*(ctypes.cast(getattr(h, f), ctypes.c_void_p).value for f in (
-            "regcn_embedding", "regcn_embedding_grad_workspace_bytes", "regcn_embedding_grad", "regcn_last_error_string")))
+            "regcn_embedding", "regcn_embedding_grad_workspace_bytes", "regcn_embedding_grad",
+            "regcn_kreduce_workspace_floats", "regcn_kreduce_gemm_f32", "regcn_last_error_string")))
         _node = m
     return _node
 

@@ -39,6 +39,11 @@ BWD = dict(log0=0, exp0=1, project=2, apply_radius=3, radius=4, mobius=5)
 FWD = dict(log0="regcn_log0_f32", exp0="regcn_exp0_f32", project="regcn_project_f32")
 
 
+def _transformed():
+    """Forward-mode differentiation or a torch.func transform is under way."""
+    return forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+
+
 def needs_grad(*ts):
     return torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in ts)
 
@@ -335,14 +340,14 @@ class _Centroid(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------- sums that replay
-SUM_STAGE = 4096
+SUM_WHOLE, SUM_STAGE = 32768, 4096
 
 
 def sum_last(x):
-    """x.sum(-1) in stages of SUM_STAGE elements.  torch sums many elements to one (131,072 and more measured) on
-    several workgroups and clears their tickets with a memset; in a replayed HIP graph such a sum returned
-    wrong values from the second replay on.  Up to 65,536 to one it stays in one workgroup."""
-    while x.shape[-1] > SUM_STAGE:
+    """x.sum(-1), of more than SUM_WHOLE elements in stages of SUM_STAGE.  torch sums many elements to one (131,072 and
+    more measured) on several workgroups and clears their tickets with a memset; in a replayed HIP graph such a
+    sum returned wrong values from the second replay on.  Up to 65,536 to one it stays in one workgroup."""
+    while x.shape[-1] > SUM_WHOLE:
         n = x.shape[-1]
         whole = n // SUM_STAGE * SUM_STAGE
         parts = x[..., :whole].unflatten(-1, (-1, SUM_STAGE)).sum(-1)
@@ -379,6 +384,19 @@ def sum_to(x, shape):
 
 class _Spread(torch.autograd.Function):
     """t.expand(shape), whose gradient is `sum_to` t's shape."""
+
+    @staticmethod
+    def forward(ctx, t, shape):
+        ctx.small = t.shape
+        return t.expand(shape)
+
+    @staticmethod
+    def backward(ctx, g):
+        return sum_to(g, ctx.small), None
+
+
+class _SpreadTransformed(torch.autograd.Function):
+    """The same under forward-mode differentiation and torch.func's transforms (its context costs 8 us a call)."""
     generate_vmap_rule = True
 
     @staticmethod
@@ -401,7 +419,9 @@ class _Spread(torch.autograd.Function):
 def spread(t, shape):
     """t broadcast to a shape, for a parameter that many rows share: torch's own broadcasting, but the gradient's sum
     replays in a HIP graph.  A Python number or None stays what it is."""
-    return _Spread.apply(t, torch.Size(shape)) if torch.is_tensor(t) else t
+    if not torch.is_tensor(t):
+        return t
+    return (_SpreadTransformed if _transformed() else _Spread).apply(t, torch.Size(shape))
 
 
 # ------------------------------------------------------------------------- cross entropy
@@ -615,28 +635,12 @@ def linear(layer, x):
     return layer(x)
 
 
-class _GruGates(torch.autograd.Function):
-    """A GRU cell's gates and new state from its two products; the bias gradients on `colsum`."""
-
-    @staticmethod
-    def forward(ctx, gi, gh, h, b_ih, b_hh):
-        out, ws = torch.ops.aten._thnn_fused_gru_cell(gi, gh, h, b_ih, b_hh)
-        ctx.save_for_backward(ws)
-        return out
-
-    @staticmethod
-    def backward(ctx, gy):
-        di, dh, dx = torch.ops.aten._thnn_fused_gru_cell_backward(gy.contiguous(), ctx.saved_tensors[0], False)[:3]
-        need = ctx.needs_input_grad
-        return di, dh, dx, colsum(di) if need[3] else None, colsum(dh) if need[4] else None
-
-
 def gru_cell(cell, x, h):
     """cell(x, h) for an nn.GRUCell (the relation GRU, hyperbolic_model.py:815-823): torch's products and fused gates.
-    With gradients its biases' sums over the rows (2R x 3d) are those of `colsum`."""
+    With gradients the biases' sums over the rows (2R x 3d) are those of `colsum` (csrc/node.cpp)."""
     if x.is_cuda and x.dim() == 2 and x.dtype == torch.float32 and cell.bias and needs_grad(x, h, *cell.parameters()):
-        return _GruGates.apply(torch.mm(x, cell.weight_ih.t()), torch.mm(h, cell.weight_hh.t()), h.contiguous(), cell.bias_ih,
-                               cell.bias_hh)
+        return _lib.node().gru_gates(torch.mm(x, cell.weight_ih.t()), torch.mm(h, cell.weight_hh.t()), h.contiguous(), cell.bias_ih,
+                                     cell.bias_hh)
     return cell(x, h)
 
 
@@ -897,7 +901,7 @@ def embedding(table, idx, scale=1.0, padding_idx=None):
     idx = idx.contiguous()
     if table.shape[1] > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < table.shape[1]:
         table = table.contiguous()
-    transformed = forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+    transformed = _transformed()
     if not transformed and _lib.EVENT_TRACE is None:
         return _lib.node().lookup(table, idx, scale, pad)
     if transformed or needs_grad(table):

@@ -111,7 +111,7 @@ class Muon(torch.optim.Optimizer):
         d = grad + momentum * buf          (nesterov; otherwise buf)
         p = (1 - lr * weight_decay) * p - lr * sqrt(max(1, rows / cols)) * orthogonalize(d)
 
-    One call of `orthogonalize` serves all the parameters of a group (per device).  The momentum and the step
+    One call of `orthogonalize` serves all the parameters of a group (per device; `full_fp32` as there).  The momentum and the step
     are fp32 whatever the parameter's type: a 16-bit parameter is rounded once, at the end.  Parameters without a
     gradient are left alone; sparse gradients are refused.  The step holds no host synchronisation, so a
     training step with it can be captured in a HIP graph (training.GraphedSteps)."""

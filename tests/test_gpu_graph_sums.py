@@ -46,7 +46,7 @@ def replays_as_eager(step, leaves, times=4):
                 k, i, float((o - w).abs().max()), float(w.abs().max()))
 
 
-@pytest.mark.parametrize("n", [4097, 131072, 1000003])
+@pytest.mark.parametrize("n", [4097, 32768, 32769, 131072, 1000003])
 def test_totals(n):
     x = torch.randn(n, 3, device=DEV)
     replays_as_eager(lambda: [A.total(x), A.total(x[:, 1]), A.sum_last(x.t())], [x])
@@ -209,3 +209,13 @@ def test_training_steps_hold_no_memset_nodes(encoder, decoder, extra):
     with torch.cuda.graph(graph, stream=side):
         step()
     assert _lib.graph_memset_nodes(graph) == 0
+
+
+def test_replayed_steps_draw_new_dropout_masks():
+    """A step's random numbers are the generator's next ones on every replay."""
+    x = torch.ones(4000, device=DEV)
+    steps = training.GraphedSteps(DEV)
+    masks = [steps.run("key", lambda: torch.nn.functional.dropout(x, 0.5) * 1.0).clone() for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(1500 < int((m > 0).sum()) < 2500 for m in masks)
+    assert not any(torch.equal(a, b) for i, a in enumerate(masks) for b in masks[:i])

@@ -7,10 +7,10 @@ import torch
 from regcn_amd import _lib
 from regcn_amd import autograd as A
 
-S = A.SUM_STAGE
+S, W = A.SUM_STAGE, A.SUM_WHOLE
 
 
-@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, S - 1, S, S + 1, 2 * S, 2 * S + 17, S * S + 1])
+@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, S, W - 1, W, W + 1, W + S, W + S + 17, W * S + 1])
 def test_total_is_the_sum(n):
     x = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(n)).double().requires_grad_(True)
     out = A.total(x)
@@ -19,7 +19,7 @@ def test_total_is_the_sum(n):
     assert torch.equal(x.grad, torch.ones(n, dtype=torch.float64))
 
 
-@pytest.mark.parametrize("shape", [(3, 1), (5, S + 3), (2, 3, 2 * S), (0, 7), (4, 0), (1, 3 * S + 1)])
+@pytest.mark.parametrize("shape", [(3, 1), (5, W + 3), (2, 3, W + S), (0, 7), (4, 0), (1, W + 3 * S + 1), (0, W + 1)])
 def test_sum_of_the_last_dimension(shape):
     x = torch.randint(-8, 9, shape, generator=torch.Generator().manual_seed(1)).float()
     assert torch.equal(A.sum_last(x), x.sum(-1))
@@ -29,7 +29,7 @@ def test_sum_of_the_last_dimension(shape):
 
 @pytest.mark.parametrize("small,shape", [((), (3, 5)), ((1,), (200, 7)), ((1, 1), (1, 1)), ((7,), (200, 7)), ((200, 1), (200, 7)),
                                          ((1, 7), (130, 7)), ((3, 1, 2), (4, 3, 65, 2)), ((), (0, 4)), ((4,), (0, 4)),
-                                         ((1,), (S + 5, 3))])
+                                         ((1,), (W + 5, 3)), ((3, 1), (3, W + 5))])
 def test_sum_to_is_the_gradient_of_broadcasting(small, shape):
     g = torch.randint(-8, 9, shape, generator=torch.Generator().manual_seed(0)).double()
     t = torch.zeros(small, dtype=torch.float64, requires_grad=True)

@@ -38,8 +38,12 @@ def main():
                          "and replay it (Adam capturable; the step has no host synchronisation)")
     ap.add_argument("--per-batch-encoder", action="store_true",
                     help="recompute the encoder per mini-batch (the reference loop) instead of once per sample")
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"])
+    ap.add_argument("--sorted-lookup", action="store_true")
     a = ap.parse_args()
     from regcn_amd import graph as G
+    from regcn_amd import muon, training
+    from regcn_amd.cli import Optimizers
     from regcn_amd.hyperbolic_model import HyperbolicRecurrentRGCN
     from regcn_amd.synthetic import CONFIGS, snapshot_series
     from regcn_amd.weights import bump_versions
@@ -53,7 +57,13 @@ def main():
                                 dropout=0.2, c=0.01, self_loop=True, layer_norm=False, input_dropout=0.2,
                                 hidden_dropout=0.2, feat_dropout=0.2, entity_prediction=True, relation_prediction=True,
                                 use_cuda=True, gpu=0, radius_target=rt, radius_msg_gamma=0.15).to(dev).train()
-    opt = torch.optim.Adam(m.parameters(), lr=1e-3, weight_decay=1e-5, capturable=a.graph, fused=True)
+    adam = dict(lr=1e-3, weight_decay=1e-5, capturable=a.graph, fused=True)
+    training.use_sorted_lookup(m, a.sorted_lookup)
+    if a.optimizer == "muon":
+        mats, rest = muon.split_parameters(m)
+        opt = Optimizers(muon.Muon(mats, weight_decay=1e-5), torch.optim.Adam(rest, **adam))
+    else:
+        opt = torch.optim.Adam(m.parameters(), **adam)
     snaps = snapshot_series(1, V, R, T + 8, per)
     graphs = [G.build_sub_graph(V, R, s, True, dev) for s in snaps]
     samples = [(graphs[i:i + T], torch.from_numpy(snaps[i + T]).to(dev)) for i in range(8)]
