@@ -610,8 +610,8 @@ __global__ __launch_bounds__(THR, 2) void k_poly(Job job) {
   const Parts<PAD> w(q);
   const int nt = w.mp / T;
   const char* A = q.ws + w.A;
-  symmetric<S>(PAD == 64 && q.fp32, symmetric_piece(wg, nt, q.poly.full, q.poly.splits, T == 128), q.poly.splits, A, (int64_t)w.mp * 4, w.mp / KSTEP, A,
-               job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
+  symmetric<S>(PAD == 64 && q.fp32, symmetric_piece(wg, nt, q.poly.full, q.poly.splits, T == 128), q.poly.splits, A, (int64_t)w.mp * 4,
+               w.mp / KSTEP, A, job.b * (EB / EX), job.c * (EB / EX / EX), q.ws + w.B, (int64_t)w.mp * 4, (float*)(q.ws + w.split),
                nt * (nt + 1) / 2 - q.poly.full, lds);
 }
 template <int PAD, int T>

@@ -23,7 +23,8 @@
 // k_sample: a workgroup takes a row of up to 32768 scores, which stay in its LDS (one read of them; in
 // registers, the compiler spilled them around the exponentials).  What bounds it is the issue of vector
 // instructions, about 90 per score with top_p: 30 for its exponential (a second one for the scores it keeps), the
-// rest for loads, bins and sums.  3080 x 23033, p = 0.9: 320 us, its 284 MB would take 60.
+// rest for loads, bins and sums.  3080 x 23033, p = 0.9: 319 us again and again on one input, 349 on inputs that change, whose
+// 284 MB would take 60.
 // k_spread_*: longer rows are cut into segments of 8192 scores, a workgroup each, in launches that pass
 // histograms, the bin's members and the segments' sums through a workspace.
 #include "elem.h"
@@ -449,7 +450,7 @@ struct LdsRow {
   }
   // Weights of what a cut keeps of them: where that is up to a quarter of the wave's scores (as the first four of each lane's
   // consecutive ones tell), each lane takes its own one after the other; else all the wave's, four at a time.
-  // (3080 x 23033: p = 0.9 346 -> 320 us, k = 500 and p = 0.9 390 -> 343 by the sums and -> 304 by the bins; p = 0.999
+  // (3080 x 23033 on one input: p = 0.9 346 -> 320 us, k = 500 and p = 0.9 390 -> 343 by the sums and -> 304 by the bins; p = 0.999
   // 348 -> 356, and 384 without the second way.)
   __device__ __forceinline__ bool few(const Cut& cut) const {
     if (!(cut.s > LOWEST)) return false;

@@ -596,10 +596,9 @@ def kreduce_mm(a, b, a_kmajor, c0=None, b_kmajor=True):
 def colsum(x):
     """x.sum(0) of a 2-D fp32 device tensor on regcn_kreduce_gemm_f32 (ones^T x: K = rows split
     over workgroups, partials summed by a second launch in a fixed order).  torch's column sum
-    of a tall matrix finishes in the kernel's last workgroup after an atomic ticket, reading
-    the other workgroups' partials through the XCDs' separate L2s; in replayed HIP graphs it
-    returned different sums for the same input (tools/graphdbg3.py: the time-gate bias
-    gradient), so the training backward sums columns here."""
+    of a tall matrix finishes in the kernel's last workgroup after an atomic ticket that a memset
+    clears; in replayed HIP graphs it returned different sums for the same input
+    (tools/graphdbg3.py: the time-gate bias gradient), so the training backward sums columns here."""
     x = x.contiguous().float()
     ones = torch.ones(x.shape[0], 1, device=x.device, dtype=torch.float32)
     return kreduce_mm(ones, x, True).reshape(x.shape[1])
