@@ -23,7 +23,8 @@
 // What the halves do not keep: X's 2^-37 is absolute, so a row of G that is 1e-4, 1e-5 or 1e-6 of the others is off by 4e-6,
 // 4e-5, 4e-4 of itself (fp32: 3e-7), at any number of steps.  Of the whole matrix that is nothing until the small
 // rows have grown by a^steps: the halves' error, modelled in 64 bits over rows of 1 to 1e-8, is 0.3 to 0.7 of fp32's up to 8
-// steps, 4 times it at 10, 40 at 12.  So more than 8 steps take fp32 operands, and a caller may ask for them (REGCN_FULL_FP32).
+// steps, 4 times it at 10, 40 at 12.  So more than 8 steps take fp32 operands, and a caller may ask for them (REGCN_FULL_FP32): 8 steps of 200 x 200
+// then take 214 us for 164, of 1333 x 777 576 for 341, of 4096 x 4096 16.9 ms for 6.0.
 //
 // Layout of an operand: rows of 8-element groups, each group 8 hi then 8 lo halves (or 8 fp32): a tile's k-step of
 // 32 is one 128-byte line of a row.  Rows and columns are padded to the tile with zeros, which
