@@ -360,6 +360,11 @@ def total(x):
     return sum_last(x.reshape(-1))
 
 
+def mean(x):
+    """x.mean(), as `sum_last`."""
+    return x.mean() if x.numel() <= SUM_WHOLE else total(x) / x.numel()
+
+
 def sum_to(x, shape):
     """x summed to a shape that broadcasts to its own, as `sum_last`.  Sums down columns go in stages of 64
     rows: torch splits those earlier (3080 x 200 measured wrong in replays, 1025 x 64 not)."""
@@ -526,7 +531,7 @@ def hyp_ce_loss(q, cand, target, c, bias=None, scale=None, margin=None, reductio
     loss = _HypCE.apply(q, cand, bias, scale, margin, target, _cf(c))
     per_query = reduction == "none"
     if not per_query:
-        loss = loss.mean()
+        loss = mean(loss)
     if _c_grad(c):
         loss = loss + _ce_c_term(q, cand, target, c, bias, scale, margin, per_query=per_query)
     return loss

@@ -117,7 +117,9 @@ class Muon(torch.optim.Optimizer):
     One call of `orthogonalize` serves all the parameters of a group (per device; `full_fp32` as there).  The momentum and the step
     are fp32 whatever the parameter's type: a 16-bit parameter is rounded once, at the end.  Parameters without a
     gradient are left alone; sparse gradients are refused.  The step holds no host synchronisation, so a
-    training step with it can be captured in a HIP graph (training.GraphedSteps)."""
+    training step with it can be captured in a HIP graph (training.GraphedSteps) once each parameter has taken a step: a
+    momentum buffer made within a capture would be cleared by every replay, and is refused.  A capture keeps the
+    settings (lr and the others) that it was made with."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS,
                  eps=1e-7, full_fp32=False):
@@ -146,7 +148,7 @@ class Muon(torch.optim.Optimizer):
         # the base class casts a state to its parameter's type; the momentum stays fp32
         keys = [k for g in state_dict["param_groups"] for k in g["params"]]
         for k, p in zip(keys, (p for g in self.param_groups for p in g["params"])):
-            if k in state_dict["state"]:
+            if "momentum_buffer" in state_dict["state"].get(k, {}):
                 self.state[p]["momentum_buffer"] = state_dict["state"][k]["momentum_buffer"].to(
                     device=p.device, dtype=torch.float32, copy=True)
 
@@ -172,6 +174,8 @@ class Muon(torch.optim.Optimizer):
         for p in ps:
             st = self.state[p]
             if "momentum_buffer" not in st:
+                if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a parameter's first Muon step cannot be captured: run one before the capture")
                 st["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
             bufs.append(st["momentum_buffer"])
         mu, lr = group["momentum"], group["lr"]

@@ -219,3 +219,42 @@ def test_replayed_steps_draw_new_dropout_masks():
     torch.cuda.synchronize()
     assert all(1500 < int((m > 0).sum()) < 2500 for m in masks)
     assert not any(torch.equal(a, b) for i, a in enumerate(masks) for b in masks[:i])
+
+
+def test_loss_of_many_queries():
+    """The mean over 140,000 queries of 40 candidates."""
+    g = torch.Generator().manual_seed(0)
+    q, cand = ((torch.randn(n, 8, generator=g) * 0.3).to(DEV).requires_grad_(True) for n in (140000, 40))
+    target = torch.randint(0, 40, (140000,), generator=g).to(DEV)
+    one = torch.ones((), device=DEV)
+
+    def step():
+        loss = A.hyp_ce_loss(q, cand, target, 0.01, scale=one, margin=one)
+        return [loss.detach(), *torch.autograd.grad(loss, [q, cand])]
+    replays_as_eager(step, [q, cand])
+
+
+def test_muon_refuses_its_first_step_in_a_capture():
+    """A momentum buffer made there would be cleared by every replay; after an eager step the capture carries it on."""
+    p, ref = (torch.randn(40, 30, generator=torch.Generator().manual_seed(1)).to(DEV).requires_grad_(True) for _ in range(2))
+    grad = torch.randn(40, 30, device=DEV)
+    opt, ref_opt = muon.Muon([p]), muon.Muon([ref])
+    p.grad, ref.grad = grad.clone(), grad.clone()
+    side = torch.cuda.Stream()
+    with pytest.raises(RuntimeError, match="first Muon step"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            opt.step()
+    torch.cuda.synchronize()
+    assert not opt.state[p]
+    for _ in range(5):
+        ref_opt.step()
+    with torch.cuda.stream(side):
+        opt.step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step()
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p, ref) and torch.equal(opt.state[p]["momentum_buffer"], ref_opt.state[ref]["momentum_buffer"])

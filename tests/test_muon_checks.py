@@ -90,3 +90,12 @@ def test_more_steps_take_fp32_operands():
         assert call(m, steps) == -1 and b"workspace" in lib.regcn_last_error_string()
     assert size(mats(200, 1 | _lib.FULL_FP32)) > 0 and size(mats(200, 3 | _lib.FULL_FP32)) == 0
     assert size(mats(64, 0)) == size(mats(64, _lib.FULL_FP32))
+
+
+def test_a_state_without_momentum_loads():
+    """Of a parameter that has not stepped yet."""
+    opt = muon.Muon([torch.zeros(2, 3, requires_grad=True)])
+    opt.state[opt.param_groups[0]["params"][0]] = {}
+    again = muon.Muon([torch.zeros(2, 3, requires_grad=True)])
+    again.load_state_dict(opt.state_dict())
+    assert not any(again.state.values())

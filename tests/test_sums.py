@@ -103,3 +103,12 @@ def test_graph_entry_refuses():
     assert _lib.lib().regcn_graph_memset_nodes(None, ctypes.byref(n)) < 0
     assert _lib.lib().regcn_graph_memset_nodes(ctypes.byref(n), None) < 0
     assert b"graph_memset_nodes" in _lib.lib().regcn_last_error_string()
+
+
+@pytest.mark.parametrize("n", [1, 5, W, W + 1, 4 * W])
+def test_mean(n):
+    x = torch.randint(-8, 9, (n,), generator=torch.Generator().manual_seed(n)).double().requires_grad_(True)
+    out = A.mean(x)
+    assert abs(float(out.detach()) - float(x.detach().sum()) / n) <= 2.0 ** -52 * 8
+    out.backward()
+    assert torch.equal(x.grad, torch.full((n,), 1.0 / n, dtype=torch.float64))
